@@ -50,6 +50,10 @@ typedef enum { PS_DTYPE_FP16 = 0, PS_DTYPE_BF16 = 1, PS_DTYPE_FP32 = 2 } ps_dtyp
 /* KV-cache element type (ps_paged_problem.kv_cache_dtype). */
 #define PS_KV_AUTO 0      /* the problem's dtype */
 #define PS_KV_FP8_E4M3 1  /* e4m3fn codes (uint8), per-tensor scales k_scale / v_scale */
+#define PS_KV_NVFP4 2     /* e2m1 codes, an e4m3 scale per 16 dims, per-tensor scales (ps_kv_append_nvfp4) */
+
+/* Bytes of one token of one head (128 dims) in an nvfp4 cache. */
+#define PS_NVFP4_ROW_BYTES 72
 
 int ps_abi_version(void);
 const char* ps_last_error(void);
@@ -129,7 +133,8 @@ typedef struct {
   const void* new_value;
   int64_t new_value_stride_token, new_value_stride_head;
   const int64_t* slot_mapping;
-  /* KV-cache element type, PS_KV_AUTO (0) or PS_KV_FP8_E4M3.  An fp8 cache
+  /* KV-cache element type: PS_KV_AUTO (0), PS_KV_FP8_E4M3 or PS_KV_NVFP4 (its
+     layout and strides: ps_kv_append_nvfp4).  An fp8 cache
      holds e4m3(x / scale) codes (ps_kv_append_fp8, or the fused append) --
      vLLM's kv_cache_dtype "fp8" with layer._k_scale / _v_scale; its strides
      are in bytes.  ps_paged_decode takes it; chunked prefill attends over
@@ -162,7 +167,34 @@ int ps_kv_append_fp8(const void* key, int64_t key_stride_token, int64_t key_stri
                      const float* v_scale, int32_t* status, void* stream);
 
 /*
- * The pages of an fp8 cache that a batch of sequences reads, dequantized
+ * KV append into a 4-bit (nvfp4) cache: a row's 16-dim blocks are stored as
+ *   scale = e4m3(max|x| / (6 * g)),  codes = e2m1(x / (scale * g))
+ * with g = k_scale for the key and v_scale for the value (device fp32
+ * scalars > 0, NULL = 1.0; products and quotients rounded to fp32, then to
+ * the nearest code, ties to even, saturating), slot < 0 skipped.  Attention
+ * reads e2m1 * scale * g.  A block whose scale rounds to zero stores zeros; a
+ * block with a NaN reads as NaN; infinities saturate.  (vLLM's
+ * kv_cache_dtype "nvfp4": the same 72 bytes per token and head,
+ * vllm/utils/torch_utils.py:415-417.)
+ *
+ * Caches: uint8 [num_blocks, num_kv_heads, block_size, 72], block_size a
+ * multiple of 16.  The 16 tokens of a page of one head are one opaque
+ * 1152-byte tile, contiguous, in the decode kernel's order (csrc/nvfp4.cuh);
+ * the caches' base and their block and head strides (bytes) are multiples of
+ * 16.  In ps_paged_problem such a cache has cache_stride_slot = 72.
+ * key/value: fp16 or bf16 (dtype), rows 16-byte aligned; head_size 128.  No
+ * two tokens of a call may share a slot >= 0 (the row's contents would be a
+ * mixture of both).
+ */
+int ps_kv_append_nvfp4(const void* key, int64_t key_stride_token, int64_t key_stride_head, const void* value,
+                       int64_t value_stride_token, int64_t value_stride_head, void* key_cache, void* value_cache,
+                       int64_t cache_stride_block, int64_t cache_stride_head, int64_t num_blocks,
+                       const int64_t* slot_mapping, int64_t num_tokens, int32_t num_kv_heads, int32_t head_size,
+                       int32_t block_size, int32_t dtype, const float* k_scale, const float* v_scale,
+                       int32_t* status, void* stream);
+
+/*
+ * The pages of an fp8 or nvfp4 cache that a batch of sequences reads, dequantized
  * into a 16-bit scratch cache, for the entry points that take 16-bit pages
  * (chunked prefill over an fp8 cache): page p < ceil(seq_lens[b] /
  * block_size) of sequence b -- cache block block_table[b * stride + p] --
@@ -170,8 +202,8 @@ int ps_kv_append_fp8(const void* key, int64_t key_stride_token, int64_t key_stri
  * ([num_seqs * max_pages, block_size, num_kv_heads, 128], problem->dtype),
  * each element code * scale rounded to that dtype.  Other scratch blocks are
  * left untouched; attend over the scratch with the block table
- * [b][p] = b * max_pages + p.  Uses the problem's fp8 cache (contiguous
- * blocks), block table, seq_lens, num_seqs, shape, dtype, k_scale / v_scale
+ * [b][p] = b * max_pages + p.  Uses the problem's fp8 (contiguous blocks) or
+ * nvfp4 cache, block table, seq_lens, num_seqs, shape, dtype, k_scale / v_scale
  * and status (nullable).
  */
 int ps_kv_dequant_gather(const ps_paged_problem* problem, int32_t max_pages, void* out_key,
@@ -201,6 +233,39 @@ int64_t ps_paged_decode_workspace_size(int32_t num_seqs, int32_t num_q_heads,
  */
 int ps_paged_decode(const ps_paged_problem* problem, void* workspace, int64_t workspace_bytes,
                     void* stream);
+
+/*
+ * Score modifiers of ps_paged_decode_mod and ps_chunked_prefill_mod.  With
+ * i the position of a query row in its sequence (seq_len - q_len + row) and j
+ * a key's, the attention's score is
+ *   z = softmax_scale * k_scale * (q . k)
+ *   z = cap * tanh(z / cap)             logits_soft_cap > 0
+ *   z = z - alibi_slopes[h] * |i - j|   alibi_slopes given
+ * over the visible keys max(0, i - window_left, key_start[row]) <= j <=
+ * max(i, prefix_lens[b] - 1), j < seq_len (each bound only where given), in
+ * the place of the plain causal attention of ps_paged_decode and
+ * ps_chunked_prefill.  A row that sees no key gets output 0 and LSE -inf.
+ * They are what vLLM's FlashAttention backend passes on as softcap,
+ * alibi_slopes and window_size (flash_attn.py:796-817), and the masks of packed
+ * documents (key_start: the first key of the row's document) and of a
+ * bidirectional prefix.  Pages below a sequence's visible range are neither
+ * read nor looked up in the block table by the decode; the prefill skips them
+ * for each pair of 128-row tiles.  Values of cached keys that a row of such a
+ * pair sees must be finite for every row of the pair (0 * inf).
+ */
+typedef struct {
+  float logits_soft_cap;      /* 0: no cap */
+  const float* alibi_slopes;  /* device [num_q_heads], NULL: no bias */
+  int32_t window_left;        /* < 0: no window */
+  const int32_t* key_start;   /* device, per query row (num_tokens entries), NULL: 0 */
+  const int32_t* prefix_lens; /* device [num_seqs], NULL: causal.  A decode row sees
+                                 every key up to its own already: no effect there */
+} ps_score_mod;
+
+/* ps_paged_decode with score modifiers, over 16-bit, fp8 and nvfp4 caches, the
+   fused append included (its token is written even where the masks hide it). */
+int ps_paged_decode_mod(const ps_paged_problem* problem, const ps_score_mod* mod, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 /*
  * Paged decode with library-owned scratch memory.  No counterpart in the
@@ -333,6 +398,11 @@ int ps_chunked_prefill(const ps_paged_problem* problem, void* stream);
  */
 int ps_chunked_prefill_ws(const ps_paged_problem* problem, void* workspace,
                           int64_t workspace_bytes, void* stream);
+
+/* ps_chunked_prefill_ws with score modifiers.  The workspace may be NULL (0
+   bytes): the units are then assigned round-robin, as in ps_chunked_prefill. */
+int ps_chunked_prefill_mod(const ps_paged_problem* problem, const ps_score_mod* mod, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 /*
  * Decode context parallelism (DCP).  The `world` ranks of a DCP group (one

@@ -61,9 +61,10 @@ extern "C" int ps_paged_decode_static_scratch(const ps_paged_problem* pr, void* 
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return ps_set_last_error(PS_ERR_CUDA, "no CUDA device");
-  // the scratch this problem's kernel needs (16-bit and fp8 caches differ)
+  // the scratch this problem's kernel needs (it depends on the cache dtype)
   const int64_t need = ps_decode_workspace_bytes(pr->num_seqs, pr->num_q_heads, pr->num_kv_heads, sms, 0,
-                                                 pr->kv_cache_dtype == PS_KV_FP8_E4M3 ? 1 : 0);
+                                                 pr->kv_cache_dtype == PS_KV_FP8_E4M3 ? 1 : 0,
+                                                 pr->kv_cache_dtype == PS_KV_NVFP4 ? 1 : 0);
   if (need > kStaticScratchBytes)
     return ps_set_last_error(PS_ERR_WORKSPACE,
                              "problem needs more decode scratch than the library's static 16 MiB "

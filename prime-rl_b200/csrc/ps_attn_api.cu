@@ -133,11 +133,11 @@ struct DecodeWorkspaceLayout {
 };
 
 DecodeWorkspaceLayout decode_layout(int num_seqs, int num_q_heads, int num_kv_heads, int sm_count,
-                                    bool cascade, bool fp8 = false) {
+                                    bool cascade, bool fp8 = false, bool fp4 = false) {
   const int group = num_q_heads / num_kv_heads;
   const int kg = (group <= 8 && !cascade) ? 8 : 16;
   const int64_t slots =
-      ps_decode_partial_slots(num_seqs, num_kv_heads, sm_count, cascade ? 1 : 0, fp8 ? 1 : 0);
+      ps_decode_partial_slots(num_seqs, num_kv_heads, sm_count, cascade ? 1 : 0, fp8 ? 1 : 0, fp4 ? 1 : 0);
   const int64_t counter_bytes = static_cast<int64_t>(ps::kDecodeMaxSeqs) * num_kv_heads * 4;
   DecodeWorkspaceLayout l;
   l.counters_off = 256;
@@ -148,7 +148,47 @@ DecodeWorkspaceLayout decode_layout(int num_seqs, int num_q_heads, int num_kv_he
   return l;
 }
 
-int validate_problem(const ps_paged_problem* pr, bool decode) {
+// An nvfp4 cache half: the tiles of a (block, head) are contiguous, blocks and
+// heads at any stride that keeps them apart.
+int validate_nvfp4_strides(const ps_paged_problem* pr) {
+  const int64_t block_head = static_cast<int64_t>(pr->block_size) * PS_NVFP4_ROW_BYTES;
+  if (pr->cache_stride_slot != PS_NVFP4_ROW_BYTES ||
+      (pr->num_kv_heads > 1 && pr->cache_stride_head < block_head) || pr->cache_stride_head % 16 ||
+      pr->cache_stride_block % 16)
+    return fail(PS_ERR_INVALID_ARGUMENT,
+                "an nvfp4 cache is [num_blocks, num_kv_heads, block_size, %d] bytes with contiguous "
+                "(block_size, %d) tiles and strides that are multiples of 16",
+                PS_NVFP4_ROW_BYTES, PS_NVFP4_ROW_BYTES);
+  return PS_OK;
+}
+
+// ps_score_mod -> kernel parameters.  scale: the problem's softmax_scale.
+int score_mod_params(const ps_score_mod* m, float scale, ps::ScoreModParams* out) {
+  if (!m) return fail(PS_ERR_INVALID_ARGUMENT, "score modifiers are NULL");
+  if (!(m->logits_soft_cap >= 0.f) || !(m->logits_soft_cap <= 3.0e38f))
+    return fail(PS_ERR_INVALID_ARGUMENT, "logits_soft_cap must be finite and >= 0 (0: no cap)");
+  if (!aligned(m->alibi_slopes, 4) || !aligned(m->key_start, 4) || !aligned(m->prefix_lens, 4))
+    return fail(PS_ERR_INVALID_ARGUMENT, "score modifier arrays must be 4-byte aligned");
+  const float log2e = 1.4426950408889634f;
+  *out = {};
+  if (m->logits_soft_cap > 0.f) {
+    out->cap_log2 = m->logits_soft_cap * log2e;
+    out->cap_in = 2.f * log2e * scale / m->logits_soft_cap;
+    // (a cap whose constants leave fp32's normal range would turn scores into NaN)
+    if (!(out->cap_log2 >= 1.2e-38f) || !(out->cap_log2 <= 1.7e38f) || !(out->cap_in <= 3.4e38f))
+      return fail(PS_ERR_INVALID_ARGUMENT, "logits_soft_cap %g is outside the usable range",
+                  static_cast<double>(m->logits_soft_cap));
+  }
+  out->slopes = m->alibi_slopes;
+  out->window_left = m->window_left;
+  out->key_start = m->key_start;
+  out->prefix_lens = m->prefix_lens;
+  return PS_OK;
+}
+
+// nvfp4 caches are accepted where the caller says so (`nvfp4`): the decode
+// entry points that have a kernel for them.
+int validate_problem(const ps_paged_problem* pr, bool decode, bool nvfp4 = false) {
   if (!pr) return fail(PS_ERR_INVALID_ARGUMENT, "problem is NULL");
   if (pr->num_seqs < 0) return fail(PS_ERR_INVALID_ARGUMENT, "num_seqs < 0");
   if (pr->num_seqs == 0) return PS_OK;
@@ -174,12 +214,19 @@ int validate_problem(const ps_paged_problem* pr, bool decode) {
     return fail(PS_ERR_INVALID_ARGUMENT, "num_blocks out of range");
   if (pr->max_blocks_per_seq < 0 || pr->block_table_stride < pr->max_blocks_per_seq)
     return fail(PS_ERR_INVALID_ARGUMENT, "block_table_stride < max_blocks_per_seq");
-  if (pr->kv_cache_dtype != PS_KV_AUTO && pr->kv_cache_dtype != PS_KV_FP8_E4M3)
+  if (pr->kv_cache_dtype != PS_KV_AUTO && pr->kv_cache_dtype != PS_KV_FP8_E4M3 &&
+      pr->kv_cache_dtype != PS_KV_NVFP4)
     return fail(PS_ERR_INVALID_ARGUMENT, "kv_cache_dtype %d unknown", pr->kv_cache_dtype);
+  if (pr->kv_cache_dtype == PS_KV_NVFP4) {
+    if (!nvfp4) return fail(PS_ERR_UNSUPPORTED, "this entry point is not built for an nvfp4 cache");
+    const int rc = validate_nvfp4_strides(pr);
+    if (rc != PS_OK) return rc;
+  }
   // 16-byte rows for TMA / vector access (strides in cache elements)
-  const int64_t cv = pr->kv_cache_dtype == PS_KV_FP8_E4M3 ? 16 : 8;
+  const int64_t cv = pr->kv_cache_dtype != PS_KV_AUTO ? 16 : 8;
   if (!aligned(pr->key_cache, 16) || !aligned(pr->value_cache, 16) ||
-      pr->cache_stride_head % cv || pr->cache_stride_slot % cv || pr->cache_stride_block % cv)
+      pr->cache_stride_head % cv || (pr->kv_cache_dtype != PS_KV_NVFP4 && pr->cache_stride_slot % cv) ||
+      pr->cache_stride_block % cv)
     return fail(PS_ERR_INVALID_ARGUMENT, "cache base/strides must be 16-byte aligned");
   if (!aligned(pr->q, 16) || pr->q_stride_head % 8 || pr->q_stride_token % 8)
     return fail(PS_ERR_INVALID_ARGUMENT, "q base/strides must be 16-byte aligned");
@@ -192,9 +239,14 @@ int validate_problem(const ps_paged_problem* pr, bool decode) {
 
 int decode_impl(const ps_paged_problem* pr, const void* plan, int64_t plan_bytes, void* workspace,
                 int64_t workspace_bytes, void* stream, bool cascade,
-                const ps_head_gather_problem* gather = nullptr) {
-  int rc = validate_problem(pr, true);
+                const ps_head_gather_problem* gather = nullptr, const ps_score_mod* mod = nullptr) {
+  int rc = validate_problem(pr, true, !cascade && gather == nullptr);
   if (rc != PS_OK) return rc;
+  ps::ScoreModParams modp = {};
+  if (mod != nullptr) {
+    rc = score_mod_params(mod, pr->softmax_scale, &modp);
+    if (rc != PS_OK) return rc;
+  }
   if (pr->num_seqs == 0) return PS_OK;
   if (pr->num_seqs > ps::kDecodeMaxSeqs)
     return fail(PS_ERR_UNSUPPORTED, "num_seqs %d > %d per decode launch", pr->num_seqs,
@@ -214,19 +266,22 @@ int decode_impl(const ps_paged_problem* pr, const void* plan, int64_t plan_bytes
                   static_cast<long long>(ps_cascade_plan_words(pr->num_seqs) * 4));
   }
   const bool fp8 = pr->kv_cache_dtype == PS_KV_FP8_E4M3;
+  const bool fp4 = pr->kv_cache_dtype == PS_KV_NVFP4;
   if (fp8 && cascade) return fail(PS_ERR_UNSUPPORTED, "cascade decode over an fp8 cache is not built");
   const DecodeWorkspaceLayout lay =
-      decode_layout(pr->num_seqs, pr->num_q_heads, pr->num_kv_heads, sms, cascade, fp8);
+      decode_layout(pr->num_seqs, pr->num_q_heads, pr->num_kv_heads, sms, cascade, fp8, fp4);
   if (!workspace || workspace_bytes < lay.total || !aligned(workspace, 256))
     return fail(PS_ERR_WORKSPACE, "decode workspace must be >= %lld bytes, 256-byte aligned",
                 static_cast<long long>(lay.total));
-  CUtensorMap kmap, vmap;
-  rc = make_page_map(&kmap, pr->key_cache, pr->num_blocks, pr->block_size, pr->num_kv_heads,
-                     pr->cache_stride_block, pr->cache_stride_slot, pr->cache_stride_head, fp8 ? 1 : 2);
-  if (rc != PS_OK) return rc;
-  rc = make_page_map(&vmap, pr->value_cache, pr->num_blocks, pr->block_size, pr->num_kv_heads,
-                     pr->cache_stride_block, pr->cache_stride_slot, pr->cache_stride_head, fp8 ? 1 : 2);
-  if (rc != PS_OK) return rc;
+  CUtensorMap kmap, vmap;  // (nvfp4 tiles are contiguous: plain bulk copies)
+  if (!fp4) {
+    rc = make_page_map(&kmap, pr->key_cache, pr->num_blocks, pr->block_size, pr->num_kv_heads,
+                       pr->cache_stride_block, pr->cache_stride_slot, pr->cache_stride_head, fp8 ? 1 : 2);
+    if (rc != PS_OK) return rc;
+    rc = make_page_map(&vmap, pr->value_cache, pr->num_blocks, pr->block_size, pr->num_kv_heads,
+                       pr->cache_stride_block, pr->cache_stride_slot, pr->cache_stride_head, fp8 ? 1 : 2);
+    if (rc != PS_OK) return rc;
+  }
   char* ws = static_cast<char*>(workspace);
   ps::DecodeParams p = {};  // every optional feature off
   p.q = pr->q;
@@ -254,7 +309,7 @@ int decode_impl(const ps_paged_problem* pr, const void* plan, int64_t plan_bytes
   p.counters = reinterpret_cast<int32_t*>(ws + lay.counters_off);
   p.part = reinterpret_cast<float*>(ws + lay.part_off);
   p.num_part_slots =
-      ps_decode_partial_slots(pr->num_seqs, pr->num_kv_heads, sms, cascade ? 1 : 0, fp8 ? 1 : 0);
+      ps_decode_partial_slots(pr->num_seqs, pr->num_kv_heads, sms, cascade ? 1 : 0, fp8 ? 1 : 0, fp4 ? 1 : 0);
   p.pre_counters = reinterpret_cast<int32_t*>(ws + lay.pre_counters_off);
   p.cas_num_groups = nullptr;
   p.cas_seq_group = p.cas_group_first = p.cas_group_size = p.cas_group_pages = nullptr;
@@ -309,8 +364,12 @@ int decode_impl(const ps_paged_problem* pr, const void* plan, int64_t plan_bytes
     p.gather_o_sh = gather->out_stride_head * 2;
     p.gather_status = gather->status;
   }
-  const int e = ps_launch_paged_decode(p, kmap, vmap, pr->dtype == PS_DTYPE_BF16, sms,
-                                       static_cast<cudaStream_t>(stream), fp8 ? 1 : 0);
+  p.mod = modp;
+  const int bf16 = pr->dtype == PS_DTYPE_BF16;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int e = fp4   ? ps_launch_paged_decode_fp4(p, bf16, sms, s, mod != nullptr)
+                : mod ? ps_launch_paged_decode_mod(p, kmap, vmap, bf16, sms, s, fp8 ? 1 : 0)
+                      : ps_launch_paged_decode(p, kmap, vmap, bf16, sms, s, fp8 ? 1 : 0);
   if (e != 0) return cuda_fail(static_cast<cudaError_t>(e), "paged_decode launch");
   return PS_OK;
 }
@@ -320,8 +379,8 @@ int decode_impl(const ps_paged_problem* pr, const void* plan, int64_t plan_bytes
 int ps_set_last_error(int code, const char* msg) { return fail(code, "%s", msg); }
 
 int64_t ps_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int sm_count,
-                                  int cascade, int fp8) {
-  return decode_layout(num_seqs, num_q_heads, num_kv_heads, sm_count, cascade != 0, fp8 != 0).total;
+                                  int cascade, int fp8, int fp4) {
+  return decode_layout(num_seqs, num_q_heads, num_kv_heads, sm_count, cascade != 0, fp8 != 0, fp4 != 0).total;
 }
 
 extern "C" {
@@ -436,6 +495,55 @@ int ps_kv_append_fp8(const void* key, int64_t key_stride_token, int64_t key_stri
   return PS_OK;
 }
 
+int ps_kv_append_nvfp4(const void* key, int64_t key_stride_token, int64_t key_stride_head, const void* value,
+                       int64_t value_stride_token, int64_t value_stride_head, void* key_cache, void* value_cache,
+                       int64_t cache_stride_block, int64_t cache_stride_head, int64_t num_blocks,
+                       const int64_t* slot_mapping, int64_t num_tokens, int32_t num_kv_heads, int32_t head_size,
+                       int32_t block_size, int32_t dtype, const float* k_scale, const float* v_scale,
+                       int32_t* status, void* stream) {
+  if (num_tokens < 0) return fail(PS_ERR_INVALID_ARGUMENT, "num_tokens < 0");
+  if (num_tokens == 0) return PS_OK;
+  if (!key || !value || !key_cache || !value_cache || !slot_mapping)
+    return fail(PS_ERR_INVALID_ARGUMENT, "a required pointer is NULL");
+  if (dtype != PS_DTYPE_BF16 && dtype != PS_DTYPE_FP16)
+    return fail(PS_ERR_UNSUPPORTED, "nvfp4 append takes fp16 or bf16 rows (dtype %d)", dtype);
+  if (head_size != 128) return fail(PS_ERR_UNSUPPORTED, "head_size %d unsupported (128)", head_size);
+  if (num_kv_heads <= 0 || num_kv_heads > (1 << 24) || block_size <= 0 || block_size % 16 || num_blocks <= 0)
+    return fail(PS_ERR_INVALID_ARGUMENT, "non-positive shape or block_size not a multiple of 16");
+  if (!aligned(key, 16) || !aligned(value, 16) || key_stride_token % 8 || key_stride_head % 8 ||
+      value_stride_token % 8 || value_stride_head % 8)
+    return fail(PS_ERR_INVALID_ARGUMENT, "key/value rows must be 16-byte aligned");
+  if (!aligned(key_cache, 16) || !aligned(value_cache, 16) || cache_stride_block % 16 || cache_stride_head % 16 ||
+      (num_kv_heads > 1 && cache_stride_head < static_cast<int64_t>(block_size) * PS_NVFP4_ROW_BYTES))
+    return fail(PS_ERR_INVALID_ARGUMENT,
+                "an nvfp4 cache's (block_size, %d) tiles must be contiguous and 16-byte aligned",
+                PS_NVFP4_ROW_BYTES);
+  int dev = 0;
+  const int sms = sm_count_current(&dev);
+  if (sms <= 0) return fail(PS_ERR_CUDA, "no CUDA device");
+  ps::AppendArgs a = {};
+  a.key = static_cast<const char*>(key);
+  a.value = static_cast<const char*>(value);
+  a.key_cache = static_cast<char*>(key_cache);
+  a.value_cache = static_cast<char*>(value_cache);
+  a.slot_mapping = slot_mapping;
+  a.key_st = key_stride_token * 2;
+  a.key_sh = key_stride_head * 2;
+  a.val_st = value_stride_token * 2;
+  a.val_sh = value_stride_head * 2;
+  a.c_sblock = cache_stride_block;
+  a.c_shead = cache_stride_head;
+  a.num_slots = num_blocks * block_size;
+  a.num_tokens = num_tokens;
+  a.num_heads = num_kv_heads;
+  a.block_size = block_size;
+  a.status = status;
+  const int e = ps_launch_kv_append_nvfp4(a, k_scale, v_scale, dtype == PS_DTYPE_BF16, sms,
+                                          static_cast<cudaStream_t>(stream));
+  if (e != 0) return cuda_fail(static_cast<cudaError_t>(e), "kv_append_nvfp4 launch");
+  return PS_OK;
+}
+
 int64_t ps_paged_decode_workspace_size(int32_t num_seqs, int32_t num_q_heads,
                                        int32_t num_kv_heads, int32_t head_size) {
   if (num_seqs < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || head_size != 128) {
@@ -447,15 +555,22 @@ int64_t ps_paged_decode_workspace_size(int32_t num_seqs, int32_t num_q_heads,
     fail(PS_ERR_CUDA, "no CUDA device");
     return -1;
   }
-  // large enough for the 16-bit-cache and the fp8-cache kernels
+  // large enough for the kernels of every cache dtype
   const int64_t a = decode_layout(num_seqs, num_q_heads, num_kv_heads, sms, false, false).total;
   const int64_t b = decode_layout(num_seqs, num_q_heads, num_kv_heads, sms, false, true).total;
-  return a > b ? a : b;
+  const int64_t c = decode_layout(num_seqs, num_q_heads, num_kv_heads, sms, false, false, true).total;
+  return a > b ? (a > c ? a : c) : (b > c ? b : c);
 }
 
 int ps_paged_decode(const ps_paged_problem* pr, void* workspace, int64_t workspace_bytes,
                     void* stream) {
   return decode_impl(pr, nullptr, 0, workspace, workspace_bytes, stream, false);
+}
+
+int ps_paged_decode_mod(const ps_paged_problem* pr, const ps_score_mod* mod, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  if (!mod) return fail(PS_ERR_INVALID_ARGUMENT, "score modifiers are NULL");
+  return decode_impl(pr, nullptr, 0, workspace, workspace_bytes, stream, false, nullptr, mod);
 }
 
 int64_t ps_cascade_plan_bytes(int32_t num_seqs) {
@@ -598,14 +713,22 @@ int ps_chunked_prefill(const ps_paged_problem* pr, void* stream) {
   return ps_chunked_prefill_ws(pr, nullptr, 0, stream);
 }
 
-int ps_chunked_prefill_ws(const ps_paged_problem* pr, void* workspace, int64_t workspace_bytes,
-                          void* stream) {
+}  // extern "C"
+
+namespace {
+int prefill_impl(const ps_paged_problem* pr, void* workspace, int64_t workspace_bytes, void* stream,
+                 const ps_score_mod* mod) {
   if (workspace != nullptr && (workspace_bytes < 256 || !aligned(workspace, 256)))
     return fail(PS_ERR_WORKSPACE, "prefill workspace must be >= 256 bytes, 256-byte aligned");
   int rc = validate_problem(pr, false);
   if (rc != PS_OK) return rc;
   if (pr->kv_cache_dtype != PS_KV_AUTO)
     return fail(PS_ERR_UNSUPPORTED, "chunked prefill over an fp8 cache is not built");
+  ps::ScoreModParams modp = {};
+  if (mod != nullptr) {
+    rc = score_mod_params(mod, pr->softmax_scale, &modp);
+    if (rc != PS_OK) return rc;
+  }
   if (pr->num_seqs == 0 || pr->num_tokens == 0) return PS_OK;
   if (pr->num_tokens < 0 || pr->num_tokens > INT32_MAX)
     return fail(PS_ERR_INVALID_ARGUMENT, "num_tokens out of range");
@@ -626,7 +749,7 @@ int ps_chunked_prefill_ws(const ps_paged_problem* pr, void* workspace, int64_t w
   rc = make_page_map(&vmap, pr->value_cache, pr->num_blocks, pr->block_size, pr->num_kv_heads,
                      pr->cache_stride_block, pr->cache_stride_slot, pr->cache_stride_head);
   if (rc != PS_OK) return rc;
-  ps::PrefillParams p;
+  ps::PrefillParams p = {};
   p.block_table = pr->block_table;
   p.bt_stride = pr->block_table_stride;
   p.max_blocks_per_seq = pr->max_blocks_per_seq;
@@ -652,10 +775,28 @@ int ps_chunked_prefill_ws(const ps_paged_problem* pr, void* workspace, int64_t w
   // dynamic unit scheduling: two counters in the workspace's reserved header
   // (bytes 16..23; the decode uses bytes 0..3 of the same header)
   p.sched = workspace != nullptr ? reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + 16) : nullptr;
-  const int e = ps_launch_chunked_prefill(p, qmap, kmap, vmap, pr->dtype == PS_DTYPE_BF16, sms,
-                                          static_cast<cudaStream_t>(stream));
+  p.mod = modp;
+  const int e = mod != nullptr
+                    ? ps_launch_chunked_prefill_mod(p, qmap, kmap, vmap, pr->dtype == PS_DTYPE_BF16, sms,
+                                                    static_cast<cudaStream_t>(stream))
+                    : ps_launch_chunked_prefill(p, qmap, kmap, vmap, pr->dtype == PS_DTYPE_BF16, sms,
+                                                static_cast<cudaStream_t>(stream));
   if (e != 0) return cuda_fail(static_cast<cudaError_t>(e), "chunked_prefill launch");
   return PS_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int ps_chunked_prefill_ws(const ps_paged_problem* pr, void* workspace, int64_t workspace_bytes,
+                          void* stream) {
+  return prefill_impl(pr, workspace, workspace_bytes, stream, nullptr);
+}
+
+int ps_chunked_prefill_mod(const ps_paged_problem* pr, const ps_score_mod* mod, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+  if (!mod) return fail(PS_ERR_INVALID_ARGUMENT, "score modifiers are NULL");
+  return prefill_impl(pr, workspace, workspace_bytes, stream, mod);
 }
 
 }  // extern "C"
@@ -980,8 +1121,9 @@ int ps_head_gather_phase(const ps_head_gather_problem* problem, int32_t phase, v
 extern "C" int ps_kv_dequant_gather(const ps_paged_problem* pr, int32_t max_pages, void* out_key,
                                     void* out_value, void* stream) {
   if (!pr) return fail(PS_ERR_INVALID_ARGUMENT, "problem is NULL");
-  if (pr->kv_cache_dtype != PS_KV_FP8_E4M3)
-    return fail(PS_ERR_INVALID_ARGUMENT, "dequantizing gather reads an fp8 cache");
+  const bool fp4 = pr->kv_cache_dtype == PS_KV_NVFP4;
+  if (pr->kv_cache_dtype != PS_KV_FP8_E4M3 && !fp4)
+    return fail(PS_ERR_INVALID_ARGUMENT, "dequantizing gather reads an fp8 or nvfp4 cache");
   if (pr->num_seqs < 0 || max_pages < 0) return fail(PS_ERR_INVALID_ARGUMENT, "negative shape");
   if (pr->num_seqs == 0 || max_pages == 0) return PS_OK;
   if (!pr->key_cache || !pr->value_cache || !pr->block_table || !pr->seq_lens || !out_key || !out_value)
@@ -990,7 +1132,12 @@ extern "C" int ps_kv_dequant_gather(const ps_paged_problem* pr, int32_t max_page
     return fail(PS_ERR_UNSUPPORTED, "scratch dtype must be fp16 or bf16 (dtype %d)", pr->dtype);
   if (pr->head_size != 128 || pr->num_kv_heads <= 0 || pr->block_size <= 0 || pr->block_size % 16)
     return fail(PS_ERR_INVALID_ARGUMENT, "shape: head_size 128, block_size a multiple of 16");
-  if (pr->cache_stride_head != 128 || pr->cache_stride_slot != static_cast<int64_t>(pr->num_kv_heads) * 128 ||
+  if (fp4) {
+    const int rc = validate_nvfp4_strides(pr);
+    if (rc != PS_OK) return rc;
+    if (!aligned(pr->key_cache, 16) || !aligned(pr->value_cache, 16))
+      return fail(PS_ERR_INVALID_ARGUMENT, "nvfp4 cache must be 16-byte aligned");
+  } else if (pr->cache_stride_head != 128 || pr->cache_stride_slot != static_cast<int64_t>(pr->num_kv_heads) * 128 ||
       pr->cache_stride_block % 16 || !aligned(pr->key_cache, 16) || !aligned(pr->value_cache, 16))
     return fail(PS_ERR_INVALID_ARGUMENT, "fp8 cache blocks must be contiguous and 16-byte aligned");
   if (!aligned(out_key, 16) || !aligned(out_value, 16))
@@ -1017,8 +1164,11 @@ extern "C" int ps_kv_dequant_gather(const ps_paged_problem* pr, int32_t max_page
   a.out_key = static_cast<char*>(out_key);
   a.out_value = static_cast<char*>(out_value);
   a.status = pr->status;
-  const int e = ps_launch_kv_dequant_gather(a, pr->dtype == PS_DTYPE_BF16, sms,
-                                            static_cast<cudaStream_t>(stream));
+  const int e = fp4 ? ps_launch_kv_dequant_gather_nvfp4(a, pr->num_kv_heads, pr->cache_stride_head,
+                                                        pr->dtype == PS_DTYPE_BF16, sms,
+                                                        static_cast<cudaStream_t>(stream))
+                    : ps_launch_kv_dequant_gather(a, pr->dtype == PS_DTYPE_BF16, sms,
+                                                  static_cast<cudaStream_t>(stream));
   return e != 0 ? cuda_fail(static_cast<cudaError_t>(e), "dequantizing gather launch") : PS_OK;
 }
 

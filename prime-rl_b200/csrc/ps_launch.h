@@ -24,6 +24,16 @@ struct AppendArgs {
   int32_t* status;
 };
 
+// Score modifiers of an attention call, derived from ps_score_mod.
+struct ScoreModParams {
+  float cap_log2;            // cap * log2(e); 0: no cap
+  float cap_in;              // 2 * log2(e) * softmax_scale / cap
+  const float* slopes;       // [num_q_heads] bias slopes; nullptr: none
+  int32_t window_left;       // keys j >= i - window_left; < 0: no window
+  const int32_t* key_start;  // [query rows] first key of the row's document; nullptr: 0
+  const int32_t* prefix_lens;  // [num_seqs] keys every row sees; nullptr: causal (prefill)
+};
+
 // Paged decode launch parameters (device-visible copy of ps_paged_problem plus
 // derived values).  Strides are in elements.
 struct DecodeParams {
@@ -82,6 +92,7 @@ struct DecodeParams {
   char* gather_out;       // [T, world * hq_local, 128] (this rank's `out` is inside it)
   int64_t gather_o_st, gather_o_sh;  // bytes
   int32_t* gather_status;
+  ScoreModParams mod;  // read by the kernels with score modifiers only
 };
 
 // Static sizing of the decode kernel, shared by the workspace-size query.
@@ -106,6 +117,15 @@ constexpr int kDecodeWarps = PS_DECODE_WARPS;           // warps per CTA
 // so the same warps and stages as the 16-bit kernel
 constexpr int kDecodeFp8Warps = PS_DECODE_FP8_WARPS;
 constexpr int kDecodeFp8Stages = PS_DECODE_FP8_STAGES;
+// 4-bit (nvfp4) caches: a unit is four pages (9 KB)
+#ifndef PS_DECODE_FP4_WARPS
+#define PS_DECODE_FP4_WARPS 8
+#endif
+#ifndef PS_DECODE_FP4_STAGES
+#define PS_DECODE_FP4_STAGES 2
+#endif
+constexpr int kDecodeFp4Warps = PS_DECODE_FP4_WARPS;
+constexpr int kDecodeFp4Stages = PS_DECODE_FP4_STAGES;
 constexpr int kDecodeMaxWarps = kDecodeWarps > kDecodeFp8Warps ? kDecodeWarps : kDecodeFp8Warps;
 constexpr int kDecodeStages = PS_DECODE_STAGES;         // pages in flight per warp
 constexpr int kDecodeCtasPerSm = PS_DECODE_CTAS_PER_SM; // persistent CTAs per SM
@@ -136,6 +156,7 @@ struct PrefillParams {
   const float* k_scale;
   const float* v_scale;
   int32_t* status;
+  ScoreModParams mod;  // read by the kernels with score modifiers only
   // dynamic unit scheduling: [0] units claimed past the grid, [1] CTAs done
   // (both zero between launches); nullptr: static round-robin
   int32_t* sched;
@@ -153,15 +174,23 @@ int ps_launch_kv_append(const ps::AppendArgs& a, int vec, int sm_count, cudaStre
 int ps_launch_paged_decode(const ps::DecodeParams& p, const CUtensorMap& kmap,
                            const CUtensorMap& vmap, int dtype_bf16, int sm_count,
                            cudaStream_t stream, int fp8_cache = 0);
+int ps_launch_paged_decode_mod(const ps::DecodeParams& p, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                               int dtype_bf16, int sm_count, cudaStream_t stream, int fp8_cache);
+// modded: with score modifiers (p.mod)
+int ps_launch_paged_decode_fp4(const ps::DecodeParams& p, int dtype_bf16, int sm_count, cudaStream_t stream,
+                               int modded);
+int ps_launch_kv_append_nvfp4(const ps::AppendArgs& a, const float* k_scale, const float* v_scale, int dtype_bf16,
+                              int sm_count, cudaStream_t stream);
 int ps_launch_kv_append_fp8(const ps::AppendArgs& a, const float* k_scale, const float* v_scale,
                             int dtype_bf16, int sm_count, cudaStream_t stream);
 
 // Split-record slots a decode launch may use: its warps plus one per unit.
-int64_t ps_decode_partial_slots(int num_seqs, int num_kv_heads, int sm_count, int cascade, int fp8 = 0);
+int64_t ps_decode_partial_slots(int num_seqs, int num_kv_heads, int sm_count, int cascade, int fp8 = 0,
+                                int fp4 = 0);
 // Workspace bytes of the decode kernel a problem of this kind launches
 // (ps_paged_decode_workspace_size returns the largest over the kinds).
 int64_t ps_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int sm_count,
-                                  int cascade, int fp8);
+                                  int cascade, int fp8, int fp4 = 0);
 
 // Shared-prefix plan (cascade_plan.cu).  Plan buffer layout in int32 words,
 // Gm = max(1, num_seqs / 2):
@@ -286,6 +315,9 @@ int ps_launch_dcp(const ps::DcpArgs& a, int which, int sm_count, cudaStream_t st
 int ps_launch_head_gather(const ps::HeadGatherArgs& a, int which, int sm_count, cudaStream_t stream);
 int ps_launch_kv_dequant_gather(const ps::DequantArgs& a, int dtype_bf16, int sm_count,
                                 cudaStream_t stream);
+// nvfp4 cache halves [num_blocks][num_heads][block_size][72]; c_shead: bytes between heads
+int ps_launch_kv_dequant_gather_nvfp4(const ps::DequantArgs& a, int num_heads, int64_t c_shead, int dtype_bf16,
+                                      int sm_count, cudaStream_t stream);
 namespace ps {
 struct MergeArgs {
   const char* p_out;
@@ -314,3 +346,6 @@ int ps_launch_cascade_plan(const ps::PlanArgs& a, cudaStream_t stream);
 int ps_launch_chunked_prefill(const ps::PrefillParams& p, const CUtensorMap& qmap,
                               const CUtensorMap& kmap, const CUtensorMap& vmap, int dtype_bf16,
                               int grid, cudaStream_t stream);
+int ps_launch_chunked_prefill_mod(const ps::PrefillParams& p, const CUtensorMap& qmap,
+                                  const CUtensorMap& kmap, const CUtensorMap& vmap, int dtype_bf16,
+                                  int grid, cudaStream_t stream);

@@ -20,8 +20,10 @@ LIB_PATH = PKG_DIR / "libps_attn.so"
 
 SOURCES = ["ps_attn_api.cu", "kv_append.cu", "paged_decode.cu", "chunked_prefill.cu",
            "paged_decode_static.cu", "cascade_plan.cu", "rope_append.cu", "dcp.cu",
-           "head_gather.cu"]
-HEADERS = ["ps_common.cuh", "ps_launch.h", "tcgen05.cuh", "peer_sync.cuh"]
+           "head_gather.cu", "paged_decode_mod.cu", "chunked_prefill_mod.cu", "nvfp4_cache.cu",
+           "paged_decode_fp4.cu"]
+HEADERS = ["ps_common.cuh", "ps_launch.h", "tcgen05.cuh", "peer_sync.cuh", "paged_decode_impl.cuh",
+           "chunked_prefill_impl.cuh", "nvfp4.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -60,7 +62,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     srcs = [str(CSRC / s) for s in SOURCES if (CSRC / s).exists()]
     tmp = target.with_suffix(".so.tmp")
     cmd = [
-        nvcc, *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
+        nvcc, *ARCH_FLAGS, "--threads", "0", "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
         "-Xcompiler", "-fPIC,-O3", "-shared", "-cudart", "static",
         f"-I{INCLUDE}", f"-I{CSRC}", "-o", str(tmp), *srcs,
     ]

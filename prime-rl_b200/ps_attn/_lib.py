@@ -30,6 +30,8 @@ PS_DTYPE_FP32 = 2
 
 PS_KV_AUTO = 0
 PS_KV_FP8_E4M3 = 1
+PS_KV_NVFP4 = 2
+PS_NVFP4_ROW_BYTES = 72
 
 ABI_VERSION = 3
 
@@ -64,6 +66,9 @@ EXPORTED_SYMBOLS = (
     "ps_paged_decode_head_gather",
     "ps_kv_dequant_gather",
     "ps_merge_attn_states",
+    "ps_kv_append_nvfp4",
+    "ps_paged_decode_mod",
+    "ps_chunked_prefill_mod",
 )
 PS_HEAD_GATHER_ROWS_OFFSET = 256
 
@@ -124,6 +129,18 @@ class PagedProblem(ctypes.Structure):
         ("kv_cache_dtype", ctypes.c_int32),
         ("k_scale", ctypes.c_void_p),
         ("v_scale", ctypes.c_void_p),
+    ]
+
+
+class ScoreMod(ctypes.Structure):
+    """Mirror of ``ps_score_mod`` in include/ps_attn.h (same field order)."""
+
+    _fields_ = [
+        ("logits_soft_cap", ctypes.c_float),
+        ("alibi_slopes", ctypes.c_void_p),
+        ("window_left", ctypes.c_int32),
+        ("key_start", ctypes.c_void_p),
+        ("prefix_lens", ctypes.c_void_p),
     ]
 
 
@@ -221,6 +238,14 @@ def _declare(lib):
         c.c_void_p, c.c_int64, c.c_int, c.c_int, c.c_int, c.c_int,  # slots, shape
         c.c_void_p, c.c_void_p,  # status, stream
     ]
+    lib.ps_kv_append_nvfp4.restype = c.c_int
+    lib.ps_kv_append_nvfp4.argtypes = [
+        c.c_void_p, c.c_int64, c.c_int64, c.c_void_p, c.c_int64, c.c_int64, c.c_void_p, c.c_void_p,
+        c.c_int64, c.c_int64, c.c_int64, c.c_void_p, c.c_int64, c.c_int32, c.c_int32, c.c_int32, c.c_int32,
+        c.c_void_p, c.c_void_p, c.c_void_p, c.c_void_p]
+    for f in (lib.ps_paged_decode_mod, lib.ps_chunked_prefill_mod):
+        f.restype = c.c_int
+        f.argtypes = [c.c_void_p, c.c_void_p, c.c_void_p, c.c_int64, c.c_void_p]
     lib.ps_kv_append_fp8.restype = c.c_int
     lib.ps_kv_append_fp8.argtypes = [
         c.c_void_p, c.c_int64, c.c_int64,  # key

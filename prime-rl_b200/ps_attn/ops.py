@@ -13,12 +13,16 @@ per decoder layer and keep their argument meaning:
 
 Tensors stay on the device; the work is enqueued on the current CUDA stream;
 nothing here synchronises or allocates except :class:`DecodeWorkspace`
-construction.  All validation failures raise :class:`ps_attn._lib.PSError` or
+construction (and :func:`dequant_gather` without ``out``).  Score modifiers (tanh cap, distance bias,
+sliding window, document and prefix masks) are a :class:`ScoreMod` passed to
+the attention calls; a 4-bit cache (:func:`nvfp4_cache_shape`) is recognised by
+its shape.  All validation failures raise :class:`ps_attn._lib.PSError` or
 ``ValueError``; there is no non-CUDA path.
 """
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 
 import torch
 
@@ -49,6 +53,97 @@ def is_fp8_cache(cache: torch.Tensor) -> bool:
     return cache.dtype in FP8_CACHE_DTYPES
 
 
+NVFP4_ROW_BYTES = _lib.PS_NVFP4_ROW_BYTES
+
+
+def nvfp4_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_size: int = 128) -> tuple:
+    """Shape of one half (K or V) of a 4-bit KV cache, a ``torch.uint8`` tensor:
+    ``(num_blocks, num_kv_heads, block_size, 72)``.  The last two dimensions are
+    an opaque sequence of 1152-byte tiles of 16 tokens (e2m1 codes and one e4m3
+    scale per 16 dims; ``csrc/nvfp4.cuh``); :func:`kv_append` writes it,
+    :func:`paged_decode` and :func:`dequant_gather` read it."""
+    if head_size != 128:
+        raise ValueError(f"nvfp4 caches hold head_size 128 (got {head_size})")
+    if block_size <= 0 or block_size % 16:
+        raise ValueError(f"block_size {block_size} must be a positive multiple of 16")
+    return (num_blocks, num_kv_heads, block_size, NVFP4_ROW_BYTES)
+
+
+def is_nvfp4_cache(cache: torch.Tensor, head_size: int = 128) -> bool:
+    """A half of a 4-bit KV cache for rows of ``head_size`` elements (an fp8
+    cache's last dimension is the head size itself)."""
+    return (cache.dtype == torch.uint8 and cache.dim() == 4 and cache.shape[-1] == NVFP4_ROW_BYTES
+            and head_size == 128)
+
+
+def _check_nvfp4(key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
+    if value_cache.dtype != torch.uint8 or key_cache.shape != value_cache.shape or \
+            key_cache.stride() != value_cache.stride():
+        raise ValueError("nvfp4: key_cache and value_cache must have the same dtype, shape and strides")
+    if key_cache.shape[2] % 16:
+        raise ValueError("nvfp4: block_size must be a multiple of 16")
+    if key_cache.stride(3) != 1 or key_cache.stride(2) != NVFP4_ROW_BYTES:
+        raise ValueError("nvfp4: the (block_size, 72) part of a cache must be contiguous")
+
+
+def _launch(device: torch.device, fn, *args) -> None:
+    """Call a C entry point with ``device`` current (the library launches on the
+    current device)."""
+    if device.index is None or torch.cuda.current_device() == device.index:
+        _lib.check(fn(*args))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args))
+
+
+@dataclass(frozen=True)
+class ScoreMod:
+    """Score modifiers of an attention call (``ps_score_mod``).
+
+    With i a query row's position in its sequence and j a key's, the score
+    ``z = softmax_scale * q.k`` becomes ``softcap * tanh(z / softcap)`` (if
+    ``softcap > 0``), then ``z - alibi_slopes[h] * |i - j|``, over the keys
+    ``max(0, i - window_left, key_start[row]) <= j <= max(i, prefix_lens[b] - 1)``
+    below the sequence's length.  A row that sees no key gives 0 and LSE -inf.
+
+    alibi_slopes: float32 [Hq]; window_left: -1 for no window (vLLM's
+    ``sliding_window - 1``); key_start: int32, one entry per query row, the
+    first key of the row's document; prefix_lens: int32 [B], the keys every row
+    of the sequence sees (prefill; no effect on a decode row, which sees all
+    keys up to its own).  Keys past a row's range may hold anything; keys that
+    one row of a sequence sees and another does not must hold finite values.
+    """
+
+    softcap: float = 0.0
+    alibi_slopes: torch.Tensor | None = None
+    window_left: int = -1
+    key_start: torch.Tensor | None = None
+    prefix_lens: torch.Tensor | None = None
+
+    def _struct(self, q: torch.Tensor, num_seqs: int) -> "_lib.ScoreMod":
+        m = _lib.ScoreMod()
+        cap = float(self.softcap)
+        if not 0.0 <= cap < float("inf"):
+            raise ValueError(f"softcap must be finite and >= 0 (got {self.softcap})")
+        m.logits_soft_cap = cap
+        w = int(self.window_left)
+        m.window_left = -1 if w < 0 else min(w, 2 ** 31 - 1)
+
+        def array(t, name, dtype, n, exact):
+            if t is None:
+                return None
+            if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or t.device != q.device:
+                raise ValueError(f"{name} must be a contiguous 1-D {dtype} tensor on {q.device}")
+            if t.shape[0] < n or (exact and t.shape[0] != n):
+                raise ValueError(f"{name} has {t.shape[0]} entries, the call needs {n}")
+            return t.data_ptr()
+
+        m.alibi_slopes = array(self.alibi_slopes, "alibi_slopes", torch.float32, q.shape[1], True)
+        m.key_start = array(self.key_start, "key_start", torch.int32, q.shape[0], False)
+        m.prefix_lens = array(self.prefix_lens, "prefix_lens", torch.int32, num_seqs, True)
+        return m
+
+
 def _scale_ptr(scale):
     if scale is None:
         return None
@@ -68,12 +163,18 @@ def kv_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
     Negative slots are skipped.  Bit-exact copy; for an fp8 cache (uint8 or
     float8_e4m3fn) the rows are stored as e4m3(x / k_scale) and
     e4m3(x / v_scale) (``reshape_and_cache_flash`` with kv_cache_dtype "fp8";
-    scales: one-element float32 device tensors, None = 1).
+    scales: one-element float32 device tensors, None = 1); for an nvfp4 cache
+    (uint8 :func:`nvfp4_cache_shape`) as e2m1 codes with an e4m3 scale per 16
+    dims under the same per-tensor scales (``ps_kv_append_nvfp4``; no two rows
+    may share a slot).
     """
     lib = _lib.load()
     _require_cuda(key, value, key_cache, value_cache, slot_mapping)
     if slot_mapping.dtype != torch.int64:
         raise ValueError("slot_mapping must be int64")
+    if key.dim() == 3 and is_nvfp4_cache(key_cache, key.shape[-1]):
+        _append_nvfp4(lib, key, value, key_cache, value_cache, slot_mapping, status, k_scale, v_scale)
+        return
     fp8 = is_fp8_cache(key_cache)
     if fp8:
         if value_cache.dtype != key_cache.dtype or key.dtype != value.dtype or \
@@ -112,6 +213,25 @@ def kv_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
         slot_mapping.data_ptr(), T, hkv, d, bs, key.element_size(),
         status.data_ptr() if status is not None else None,
         _stream_ptr(key.device)))
+
+
+def _append_nvfp4(lib, key, value, key_cache, value_cache, slot_mapping, status, k_scale, v_scale) -> None:
+    _check_nvfp4(key_cache, value_cache)
+    if key.dtype != value.dtype or key.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("nvfp4 cache: fp16/bf16 key and value rows of one dtype")
+    if key.stride(-1) != 1 or value.stride(-1) != 1 or not slot_mapping.is_contiguous():
+        raise ValueError("key/value rows and slot_mapping must be contiguous")
+    nb, hkv, bs, _ = key_cache.shape
+    T = slot_mapping.shape[0]
+    if key.shape[0] < T or value.shape[0] < T:
+        raise ValueError("key/value have fewer rows than slot_mapping")
+    if key.shape[1:] != (hkv, 128) or value.shape[1:] != (hkv, 128):
+        raise ValueError(f"key/value shape {tuple(key.shape)} does not match {hkv} kv heads of 128")
+    _launch(key.device, lib.ps_kv_append_nvfp4,
+            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
+            key_cache.data_ptr(), value_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1), nb,
+            slot_mapping.data_ptr(), T, hkv, 128, bs, _DTYPES[key.dtype], _scale_ptr(k_scale),
+            _scale_ptr(v_scale), status.data_ptr() if status is not None else None, _stream_ptr(key.device))
 
 
 def rope_kv_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -318,8 +438,13 @@ def _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
     _require_cuda(q, key_cache, value_cache, block_table, seq_lens, out, query_start_loc, lse)
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"attention dtype {q.dtype} unsupported (fp16/bf16)")
-    fp8 = is_fp8_cache(key_cache)
-    if fp8:
+    fp4 = is_nvfp4_cache(key_cache, q.shape[-1])
+    fp8 = is_fp8_cache(key_cache) and not fp4
+    if fp4:
+        _check_nvfp4(key_cache, value_cache)
+        if out.dtype != q.dtype:
+            raise ValueError("nvfp4 cache: out must have the query dtype")
+    elif fp8:
         if value_cache.dtype != key_cache.dtype or out.dtype != q.dtype:
             raise ValueError("fp8 cache: both caches fp8, out in the query dtype")
     elif key_cache.dtype != q.dtype or value_cache.dtype != q.dtype or out.dtype != q.dtype:
@@ -337,6 +462,8 @@ def _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
     if lse is not None and lse.dtype != torch.float32:
         raise ValueError("lse must be float32 [num_q_heads, num_tokens]")
     nb, bs, hkv, d = key_cache.shape
+    if fp4:
+        nb, hkv, bs, d = key_cache.shape[0], key_cache.shape[1], key_cache.shape[2], q.shape[-1]
     hq = q.shape[1]
     pr = _lib.PagedProblem()
     pr.q = q.data_ptr()
@@ -344,6 +471,8 @@ def _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
     pr.key_cache = key_cache.data_ptr()
     pr.value_cache = value_cache.data_ptr()
     pr.cache_stride_block, pr.cache_stride_slot, pr.cache_stride_head = key_cache.stride()[:3]
+    if fp4:
+        pr.cache_stride_head, pr.cache_stride_slot = key_cache.stride()[1:3]
     pr.num_blocks = nb
     pr.block_table = block_table.data_ptr()
     pr.block_table_stride = block_table.stride(0)
@@ -371,6 +500,8 @@ def _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
         pr.status = status.data_ptr()
     if fp8:
         pr.kv_cache_dtype = _lib.PS_KV_FP8_E4M3
+    elif fp4:
+        pr.kv_cache_dtype = _lib.PS_KV_NVFP4
     pr.k_scale = _scale_ptr(k_scale)
     pr.v_scale = _scale_ptr(v_scale)
     return pr
@@ -385,7 +516,8 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
                  slot_mapping: torch.Tensor | None = None,
                  cascade: CascadePlan | None = None, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None, out_address: int | None = None,
-                 head_gather: "_lib.HeadGatherProblem | None" = None) -> torch.Tensor:
+                 head_gather: "_lib.HeadGatherProblem | None" = None,
+                 score_mod: ScoreMod | None = None) -> torch.Tensor:
     """Decode attention, one query row per sequence, written into ``out``.
 
     q/out: [T, Hq, D]; caches [num_blocks, block_size, Hkv, D]; block_table
@@ -415,12 +547,23 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
     ``ps_paged_decode_head_gather`` (the group's rows land in
     ``head_gather.out`` on every rank; ``out`` only supplies shape and dtype).
     Used by :class:`ps_attn.sharding.FusedHeadGather`.
+
+    nvfp4 caches (uint8, :func:`nvfp4_cache_shape`): attention over e2m1 *
+    block scale * k_scale (v_scale); the fused append stores what
+    :func:`kv_append` stores.
+
+    ``score_mod``: a :class:`ScoreMod` (any cache dtype, with the fused append;
+    not with ``cascade`` or ``head_gather``).  Pages below a sequence's visible
+    range are neither read nor looked up.
     """
     lib = _lib.load()
     B = seq_lens.shape[0]
+    fp4 = is_nvfp4_cache(key_cache, q.shape[-1])
+    if (fp4 or score_mod is not None) and (cascade is not None or head_gather is not None):
+        raise ValueError("nvfp4 caches and score modifiers take neither a cascade plan nor the fused head gather")
     if workspace is None:
-        workspace = get_workspace(B, q.shape[1], key_cache.shape[2], key_cache.shape[3], q.device,
-                                  cascade=cascade is not None)
+        hkv, d = (key_cache.shape[1], q.shape[2]) if fp4 else (key_cache.shape[2], key_cache.shape[3])
+        workspace = get_workspace(B, q.shape[1], hkv, d, q.device, cascade=cascade is not None)
     elif workspace.max_num_seqs < B:
         raise ValueError(f"workspace sized for {workspace.max_num_seqs} sequences < {B}")
     if cascade is not None and cascade.num_seqs != B:
@@ -440,7 +583,7 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
             raise ValueError("slot_mapping must be contiguous int64")
         if new_key.dtype != q.dtype or new_value.dtype != q.dtype:
             raise ValueError("new key/value must have the query dtype")
-        hkv, d = key_cache.shape[2], key_cache.shape[3]
+        hkv, d = (key_cache.shape[1], q.shape[2]) if fp4 else (key_cache.shape[2], key_cache.shape[3])
         if new_key.shape[1:] != (hkv, d) or new_value.shape[1:] != (hkv, d):
             raise ValueError("new key/value shape does not match the cache")
         if new_key.stride(-1) != 1 or new_value.stride(-1) != 1:
@@ -462,39 +605,54 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
         _lib.check(lib.ps_paged_decode_cascade(ctypes.byref(pr), cascade.buffer.data_ptr(),
                                                cascade.nbytes, workspace.buffer.data_ptr(),
                                                workspace.nbytes, _stream_ptr(q.device)))
+    elif score_mod is not None:
+        mod = score_mod._struct(q, B)
+        _launch(q.device, lib.ps_paged_decode_mod, ctypes.byref(pr), ctypes.byref(mod),
+                workspace.buffer.data_ptr(), workspace.nbytes, _stream_ptr(q.device))
     else:
-        _lib.check(lib.ps_paged_decode(ctypes.byref(pr), workspace.buffer.data_ptr(),
-                                       workspace.nbytes, _stream_ptr(q.device)))
+        _launch(q.device, lib.ps_paged_decode, ctypes.byref(pr), workspace.buffer.data_ptr(),
+                workspace.nbytes, _stream_ptr(q.device))
     return out
 
 
 def dequant_gather(key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor,
                    seq_lens: torch.Tensor, max_pages: int, dtype: torch.dtype,
                    k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
-                   status: torch.Tensor | None = None):
-    """The pages ``seq_lens`` covers of an fp8 cache, dequantized into a
+                   status: torch.Tensor | None = None, out: tuple | None = None):
+    """The pages ``seq_lens`` covers of an fp8 or nvfp4 cache, dequantized into a
     16-bit scratch cache: returns (key, value [B * max_pages, bs, Hkv, D] of
     ``dtype``, block table [B, max_pages] int32 into them).  Pages past a
     sequence's length are left uninitialised (never read).  Without scales
-    the scratch holds the e4m3 values exactly (attend over it with the
-    scales); with them, code * scale rounded to ``dtype``."""
+    the scratch holds the e4m3 values (nvfp4: code * block scale) exactly
+    (attend over it with the scales); with them, code * scale rounded to
+    ``dtype``.  ``out``: the (key, value) scratch to write into, contiguous and
+    of that shape, instead of new tensors."""
     lib = _lib.load()
     _require_cuda(key_cache, value_cache, block_table, seq_lens)
     if not is_fp8_cache(key_cache) or value_cache.dtype != key_cache.dtype:
-        raise ValueError("dequant_gather reads an fp8 cache")
+        raise ValueError("dequant_gather reads an fp8 or nvfp4 cache")
     B = seq_lens.shape[0]
     nb, bs, hkv, d = key_cache.shape
+    if is_nvfp4_cache(key_cache):
+        nb, hkv, bs, d = key_cache.shape[0], key_cache.shape[1], key_cache.shape[2], 128
     dev = key_cache.device
-    kd = torch.empty(B * max_pages, bs, hkv, d, dtype=dtype, device=dev)
-    vd = torch.empty_like(kd)
+    if out is None:
+        kd = torch.empty(B * max_pages, bs, hkv, d, dtype=dtype, device=dev)
+        vd = torch.empty_like(kd)
+    else:
+        kd, vd = out
+        for x in (kd, vd):
+            if tuple(x.shape) != (B * max_pages, bs, hkv, d) or x.dtype != dtype or x.device != dev \
+                    or not x.is_contiguous():
+                raise ValueError(f"out must be contiguous [{B * max_pages}, {bs}, {hkv}, {d}] {dtype} on {dev}")
     bt = torch.arange(B * max_pages, dtype=torch.int32, device=dev).view(B, max_pages)
     if B == 0 or max_pages == 0:
         return kd, vd, bt
     q_like = torch.empty(1, 1, d, dtype=dtype, device=dev)
     pr = _problem(q_like, key_cache, value_cache, block_table, seq_lens, None, 1.0, q_like, None,
                   status=status, k_scale=k_scale, v_scale=v_scale)
-    _lib.check(lib.ps_kv_dequant_gather(ctypes.byref(pr), max_pages, kd.data_ptr(), vd.data_ptr(),
-                                        _stream_ptr(dev)))
+    _launch(dev, lib.ps_kv_dequant_gather, ctypes.byref(pr), max_pages, kd.data_ptr(), vd.data_ptr(),
+            _stream_ptr(dev))
     return kd, vd, bt
 
 
@@ -530,7 +688,8 @@ def chunked_prefill(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
                     status: torch.Tensor | None = None,
                     workspace: "DecodeWorkspace | None" = None,
                     k_scale: torch.Tensor | None = None,
-                    v_scale: torch.Tensor | None = None) -> torch.Tensor:
+                    v_scale: torch.Tensor | None = None,
+                    score_mod: ScoreMod | None = None) -> torch.Tensor:
     """Causal (bottom-right) varlen attention over the paged cache; any q_len >= 1.
 
     ``k_scale``/``v_scale`` (one-element float32 device tensors): the cache
@@ -542,13 +701,22 @@ def chunked_prefill(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     optional) receives PS_DEV_* bits from device-side checks.  With a
     ``workspace`` (a :class:`DecodeWorkspace` serves) the work units are
     handed out dynamically (``ps_chunked_prefill_ws``).
+
+    ``score_mod``: a :class:`ScoreMod`; its ``key_start`` is indexed like the
+    rows of ``q``, its ``prefix_lens`` like ``seq_lens``.  KV tiles that no row
+    of a pair of 128-row tiles sees are skipped.
     """
     lib = _lib.load()
     if query_start_loc is None:
         raise ValueError("chunked_prefill needs query_start_loc")
     pr = _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
                   softmax_scale, out, lse, status, k_scale=k_scale, v_scale=v_scale)
-    if workspace is not None:
+    if score_mod is not None:
+        mod = score_mod._struct(q, seq_lens.shape[0])
+        _launch(q.device, lib.ps_chunked_prefill_mod, ctypes.byref(pr), ctypes.byref(mod),
+                workspace.buffer.data_ptr() if workspace is not None else None,
+                workspace.nbytes if workspace is not None else 0, _stream_ptr(q.device))
+    elif workspace is not None:
         _lib.check(lib.ps_chunked_prefill_ws(ctypes.byref(pr), workspace.buffer.data_ptr(),
                                              workspace.nbytes, _stream_ptr(q.device)))
     else:
@@ -557,10 +725,11 @@ def chunked_prefill(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
 
 
 def paged_attention(q, key_cache, value_cache, out, query_start_loc, max_query_len, seq_lens,
-                    softmax_scale, block_table, lse=None, workspace=None):
+                    softmax_scale, block_table, lse=None, workspace=None, score_mod=None):
     """``flash_attn_varlen_func``'s paged, causal call shape: route by ``max_query_len``."""
     if max_query_len <= 1:
         return paged_decode(q, key_cache, value_cache, block_table, seq_lens, softmax_scale, out,
-                            lse=lse, query_start_loc=query_start_loc, workspace=workspace)
+                            lse=lse, query_start_loc=query_start_loc, workspace=workspace,
+                            score_mod=score_mod)
     return chunked_prefill(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
-                           softmax_scale, out, lse=lse)
+                           softmax_scale, out, lse=lse, score_mod=score_mod)
