@@ -5,8 +5,8 @@
 // A page-head is 2304 bytes (K tile + V tile) against 8192 in 16 bits, so
 // what bounds the kernel is the instruction stream that turns codes into
 // tensor-core operands, not HBM.  Hence:
-//   - the unit of work is kFp4UnitPages pages of one (sequence, kv head): one
-//     mbarrier wait, one maximum and one rescale per unit;
+//   - the unit of work is a few pages of one (sequence, kv head): one
+//     wait, one maximum and one rescale per unit;
 //   - the tile layout (nvfp4.cuh) is the fragment order: a lane's K codes are
 //     two 16-byte loads and its V codes two more, without ldmatrix;
 //   - K: the reduction dims of the 8 MMA steps are permuted so that a lane
@@ -28,21 +28,38 @@ namespace ps {
 #ifndef PS_DECODE_FP4_PAGES
 #define PS_DECODE_FP4_PAGES 4
 #endif
-constexpr int kFp4UnitPages = PS_DECODE_FP4_PAGES;  // pages of one unit
-constexpr int kFp4Warps = kDecodeFp4Warps;
+#ifndef PS_DECODE_FP4_PAGES2
+#define PS_DECODE_FP4_PAGES2 4
+#endif
 constexpr int kFp4Stages = kDecodeFp4Stages;
-constexpr int kFp4UnitTokens = kFp4UnitPages * kPageTokens;
-constexpr int kFp4StageBytes = 2 * kFp4UnitPages * kFp4TileBytes;  // K tiles, then V tiles
-static_assert(2 * kFp4UnitPages <= 32, "a lane issues one tile of a unit");
-static_assert(kFp4StageBytes % 128 == 0, "stage alignment");
+// Pages of one unit and warps of a CTA, by query-column tiles.
+template <int NT>
+__host__ __device__ constexpr int fp4_pages() {
+  return NT == 1 ? PS_DECODE_FP4_PAGES : PS_DECODE_FP4_PAGES2;
+}
+template <int NT>
+__host__ __device__ constexpr int fp4_warps() {
+  return NT == 1 ? kDecodeFp4Warps : kDecodeFp4Warps2;
+}
+template <int NT>
+__host__ __device__ constexpr int fp4_stage_bytes() {  // K tiles, then V tiles
+  return 2 * fp4_pages<NT>() * kFp4TileBytes;
+}
 
-__device__ __forceinline__ void bulk_load_hint(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar,
-                                               uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-          smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(gsrc)), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
+// 16 bytes global -> shared, asynchronous, through L2 only.
+__device__ __forceinline__ void cp_async16(uint32_t smem_dst, const void* gsrc, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(smem_dst),
+               "l"(reinterpret_cast<uint64_t>(gsrc)), "l"(policy)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t smem_dst, const void* gsrc) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(gsrc))
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
 // Query slot: unpadded rows (they are read once per segment, and the padding
@@ -54,86 +71,187 @@ __host__ __device__ constexpr int fp4_qslot_bytes() {
 }
 template <int NT>
 __host__ __device__ constexpr int fp4_smem_bytes_before_table() {
-  // stages | per-warp query slots | mbarriers
-  return kFp4Warps * kFp4Stages * (kFp4StageBytes + fp4_qslot_bytes<NT>() + 8);
+  // stages | per-warp query slots
+  return fp4_warps<NT>() * kFp4Stages * (fp4_stage_bytes<NT>() + fp4_qslot_bytes<NT>());
 }
 
-// One warp streams units [start, end) of the list.
+// Position in the list.  A segment (sequence, kv head) of P units takes P +
+// kFp4SegCost positions, the last of them empty: what its end and the next
+// segment's start cost a warp (partial rows, counter, query fragments: 4,000
+// cycles, a unit 4,400), so that the equal cut also gives equal times to warps
+// with more segment ends.  40 sequences of 2k-32k tokens, 64 / 8 heads: 120.4 us
+// without, 117.3 with 1, 119.0 with 2, 120.7 with 4.
+#ifndef PS_DECODE_FP4_SEG_COST
+#define PS_DECODE_FP4_SEG_COST 1
+#endif
+constexpr int kFp4SegCost = PS_DECODE_FP4_SEG_COST;
+struct Fp4Cursor {
+  int b, h, p, P, off;
+  int64_t v;  // position in the list
+};
+
+template <bool kMod, int kUnitTokens>
+__device__ __forceinline__ void fp4_sequence(Fp4Cursor& c, const DecodeParams& p, const int* prefix) {
+  c.P = seq_pages(prefix, c.b) - kFp4SegCost;
+  c.off = 0;
+  if constexpr (kMod) c.off = mod_first_unit(p, c.b, __ldg(p.seq_lens + c.b), kUnitTokens);
+}
+
+// Step to the next unit; c.v >= end afterwards (and nothing else of c valid)
+// when there is none before `end`.
+template <bool kMod, int kUnitTokens>
+__device__ __forceinline__ void fp4_next(Fp4Cursor& c, const DecodeParams& p, const int* prefix, int64_t end) {
+  ++c.v;
+  if (++c.p < c.P) return;
+  c.v += kFp4SegCost - (c.p - c.P);  // (a cursor placed on an empty position is past P already)
+  c.p = 0;
+  if (c.v >= end || ++c.h < p.num_kv_heads) return;
+  c.h = 0;
+  do ++c.b;
+  while (seq_pages(prefix, c.b) == 0);
+  fp4_sequence<kMod, kUnitTokens>(c, p, prefix);
+}
+
+// First unit at or after position v; v < end <= the list's length.
+template <bool kMod, int kUnitTokens>
+__device__ __forceinline__ Fp4Cursor fp4_seek(int64_t v, int64_t end, const DecodeParams& p, const int* prefix) {
+  Fp4Cursor c;
+  int lo = 0, hi = p.num_seqs - 1;  // largest b with prefix[b] * Hkv <= v
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (static_cast<int64_t>(prefix[mid]) * p.num_kv_heads <= v)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  c.b = lo;
+  c.v = v;
+  const int V = seq_pages(prefix, lo);
+  const int64_t r = v - static_cast<int64_t>(prefix[lo]) * p.num_kv_heads;
+  c.h = static_cast<int>(r / V);
+  c.p = static_cast<int>(r - static_cast<int64_t>(c.h) * V);
+  fp4_sequence<kMod, kUnitTokens>(c, p, prefix);
+  if (c.p >= c.P) {  // an empty position: the next segment's first unit
+    --c.v;
+    --c.p;
+    fp4_next<kMod, kUnitTokens>(c, p, prefix, end);
+  }
+  return c;
+}
+
+// One warp streams the units of list positions [start, end).
 template <bool kBF16, int NT, bool kMod>
 __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Tables& tb, int64_t start, int64_t end,
-                                                 int64_t gw, uint8_t* wsm, uint8_t* wq, uint64_t* wbar, int lane) {
-  constexpr int kMode = kMod ? kModded : kPlain;
+                                                 int64_t gw, uint8_t* wsm, uint8_t* wq, int lane) {
   constexpr int kRec = 8 * NT;
   constexpr int D = kFp4Stages;
-  constexpr int kUP = kFp4UnitPages;
+  constexpr int kUP = fp4_pages<NT>();
+  constexpr int kUnitTokens = kUP * kPageTokens;
+  constexpr int SB = fp4_stage_bytes<NT>();
+  static_assert(kUP % 2 == 0 && kUP <= 32, "the scale rows of a unit are copied four tiles at a time");
+  static_assert(SB % 128 == 0, "stage alignment");
   const int Hkv = p.num_kv_heads;
   const int spb = p.block_size / kPageTokens;
   const int group = p.group;
-  const int cnt = static_cast<int>(end - start);
   const float k_scale = p.k_scale ? __ldg(p.k_scale) : 1.f;
   const float v_scale = p.v_scale ? __ldg(p.v_scale) : 1.f;
   const float scale_log2 = p.scale_log2 * k_scale;
 
-  int bt_b = -1, bt_e0 = 0, bt_reg = 0;
+  // Block-table entries are held 64 at a time, [bt_e0, bt_e0 + 64) of sequence
+  // bt_b: the second half is loaded when the first comes into use, so that
+  // only a new sequence waits for its entries.
+  int bt_b = -1, bt_e0 = 0, bt_reg = 0, bt_next = 0;
   int pseg = 0;
+  // page / spb without a division: spb = block_size / 16 is in [1, 16] and a
+  // page index below 2^27, so the 2^32-scaled reciprocal, rounded up, is exact
+  const uint64_t spb_inv = ((1ull << 32) + spb - 1) / spb;
+  auto block_of = [&](int page) { return static_cast<int>((static_cast<uint64_t>(page) * spb_inv) >> 32); };
+  auto entry = [&](int b, int idx) {
+    return idx < p.max_blocks_per_seq ? __ldg(p.block_table + b * p.bt_stride + idx) : 0;
+  };
   const uint64_t kv_policy = l2_policy_evict_first();
-  // Issue the tiles of unit c into `stage`: lane u copies page u's K tile, lane
-  // kUP + u its V tile.  Pages past the sequence are not copied (their tokens
-  // are masked).
-  auto issue = [&](int stage, const Cursor& c, bool seg_start) {
+  // Issue the tiles of unit c into `stage` as one group of asynchronous copies:
+  // two 512-byte warp copies of codes per tile, and one warp copy for the
+  // scale rows (128 bytes) of four tiles.  Pages past the sequence or below the
+  // visible range are neither copied nor looked up (their tokens are masked).
+  // (Bulk copies, one per tile, cost a warp 140 cycles each to issue -- their
+  // operands are uniform, so lanes take turns -- 1,130 a unit of four pages, a
+  // quarter of its time.)
+  auto issue = [&](int stage, const Fp4Cursor& c, bool seg_start) {
     const int pg0 = (c.p + c.off) * kUP;
     int npg = kUP;
     if (c.p == c.P - 1) {  // only a sequence's last unit can be short
       const int L = max(__ldg(p.seq_lens + c.b), 0);
       npg = min(kUP, min((L + kPageTokens - 1) / kPageTokens, p.max_blocks_per_seq * spb) - pg0);
     }
-    const int e0 = pg0 / spb, e_last = (pg0 + npg - 1) / spb;
-    if (c.b != bt_b || e0 < bt_e0 || e_last >= bt_e0 + 32) {
+    int skip = 0;
+    if constexpr (kMod) skip = mod_skip_pages(p, c.b, pg0, c.p == 0);
+    const int e0 = block_of(pg0);
+    if (c.b != bt_b || e0 < bt_e0) {  // (another kv head starts over)
       bt_b = c.b;
       bt_e0 = e0;
-      const int idx = e0 + lane;
-      bt_reg = idx < p.max_blocks_per_seq ? __ldg(p.block_table + c.b * p.bt_stride + idx) : 0;
+      bt_reg = entry(c.b, e0 + lane);
+      bt_next = entry(c.b, e0 + 32 + lane);
+    } else if (e0 >= bt_e0 + 32) {
+      bt_e0 += 32;
+      bt_reg = bt_next;
+      bt_next = entry(c.b, bt_e0 + 32 + lane);
     }
-    const int which = lane / kUP;  // 0: K, 1: V, more: idle
-    const int u = lane - which * kUP;
-    int skip = 0;  // pages below the visible range are neither copied nor looked up
-    if constexpr (kMod) skip = mod_skip_pages(p, c.b, pg0, c.p == 0);
-    const bool mine = which < 2 && u >= skip && u < npg;
-    const int pg = pg0 + (mine ? u : 0);
-    const int e = pg / spb;
-    int blk = __shfl_sync(0xffffffffu, bt_reg, e - bt_e0);
-    uint64_t* bar = wbar + stage;
-    const uint32_t qbytes = seg_start ? static_cast<uint32_t>(group) * (kHeadDim * 2) : 0u;
-    if (lane == 0) mbar_arrive_expect_tx(bar, (npg - skip) * 2 * kFp4TileBytes + qbytes);
-    __syncwarp();  // expect_tx is armed before a copy can complete
-    if (mine) {
-      if (blk < 0 || blk >= p.num_blocks) {
-        set_status(p.status, PS_DEV_BLOCK_OUT_OF_RANGE);
-        blk = 0;
+    // lane u < kUP: byte offset of page u's tile in either cache half
+    const int pg = pg0 + min(lane, npg - 1), e = block_of(pg);
+    // (shuffles take the lane index modulo 32)
+    const int b_lo = __shfl_sync(0xffffffffu, bt_reg, e - bt_e0), b_hi = __shfl_sync(0xffffffffu, bt_next, e - bt_e0);
+    int blk = e - bt_e0 < 32 ? b_lo : b_hi;
+    if (blk < 0 || blk >= p.num_blocks) {
+      if (lane >= skip && lane < npg) set_status(p.status, PS_DEV_BLOCK_OUT_OF_RANGE);
+      blk = 0;
+    }
+    const int64_t tile = blk * p.c_sblock + c.h * p.c_shead + (pg - e * spb) * kFp4TileBytes;
+    const char* kbase = static_cast<const char*>(p.key_cache);
+    const char* vbase = static_cast<const char*>(p.value_cache);
+    const uint32_t dst = smem_u32(wsm + stage * SB) + lane * 16;
+#pragma unroll
+    for (int u = 0; u < kUP; ++u) {
+      const int64_t off = __shfl_sync(0xffffffffu, tile, u) + lane * 16;
+      if (u >= skip && u < npg) {
+        cp_async16(dst + u * kFp4TileBytes, kbase + off, kv_policy);
+        cp_async16(dst + u * kFp4TileBytes + 512, kbase + off + 512, kv_policy);
+        cp_async16(dst + (kUP + u) * kFp4TileBytes, vbase + off, kv_policy);
+        cp_async16(dst + (kUP + u) * kFp4TileBytes + 512, vbase + off + 512, kv_policy);
       }
-      const char* src = static_cast<const char*>(which ? p.value_cache : p.key_cache) + blk * p.c_sblock +
-                        c.h * p.c_shead + (pg - e * spb) * kFp4TileBytes;
-      bulk_load_hint(wsm + stage * kFp4StageBytes + (which * kUP + u) * kFp4TileBytes, src, kFp4TileBytes, bar,
-                     kv_policy);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * kUP; i += 4) {  // tile i + lane / 8 of K tiles, then V tiles
+      const int x = i + (lane >> 3), u = x < kUP ? x : x - kUP;
+      const int64_t off = __shfl_sync(0xffffffffu, tile, u) + kFp4CodeBytes + (lane & 7) * 16;
+      if (u >= skip && u < npg)
+        cp_async16(smem_u32(wsm + stage * SB) + x * kFp4TileBytes + kFp4CodeBytes + (lane & 7) * 16,
+                   (x < kUP ? kbase : vbase) + off, kv_policy);
     }
     if (seg_start) {
-      if (lane < group) {
-        const int qrow = p.qsl ? __ldg(p.qsl + c.b) : c.b;
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + qrow * p.q_st + (c.h * group + lane) * p.q_sh;
-        bulk_load(wq + (pseg % D) * fp4_qslot_bytes<NT>() + lane * kFp4QRowBytes, src, kHeadDim * 2, bar);
-      }
+      const int qrow = p.qsl ? __ldg(p.qsl + c.b) : c.b;
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + qrow * p.q_st + static_cast<int64_t>(c.h) * group * p.q_sh;
+      const uint32_t qdst = smem_u32(wq + (pseg % D) * fp4_qslot_bytes<NT>());
+      for (int i = lane; i < group * 16; i += 32)
+        cp_async16(qdst + i * 16, q + (i >> 4) * p.q_sh + (i & 15) * 8);
       ++pseg;
     }
+    cp_async_commit();
   };
 
-  Cursor pc = cursor_at<kMode>(start, p, tb, Hkv);
-  Cursor cc = pc;
-  const int npre = min(cnt, D);
-  for (int k = 0; k < npre; ++k) {
-    if (k > 0) cursor_next<kMode>(pc, p, tb, Hkv);
-    issue(k, pc, k == 0 || pc.p == 0);
+  Fp4Cursor pc = fp4_seek<kMod, kUnitTokens>(start, end, p, tb.prefix);
+  if (pc.v >= end) return;  // empty positions only
+  Fp4Cursor cc = pc;
+  // pc is the next unit to copy, cc the next to attend over
+#pragma unroll 1
+  for (int k = 0; k < D; ++k) {
+    if (pc.v < end) {
+      issue(k, pc, k == 0 || pc.p == 0);
+      fp4_next<kMod, kUnitTokens>(pc, p, tb.prefix, end);
+    } else {
+      cp_async_commit();
+    }
   }
-  int issued = npre;
 
   const int g = lane >> 2, t = lane & 3;
   uint32_t qf[NT][8][2];
@@ -146,16 +264,13 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
   uint4 new_row = make_uint4(0u, 0u, 0u, 0u);
   int64_t new_slot = -1;
 
-  for (int k = 0; k < cnt; ++k) {
+  for (int k = 0; cc.v < end; ++k) {
     const int stage = k % D;
-    uint8_t* st = wsm + stage * kFp4StageBytes;
-    if (!mbar_wait_bounded(wbar + stage, static_cast<uint32_t>((k / D) & 1))) {
-      if (lane == 0) set_status(p.status, PS_DEV_WAIT_TIMEOUT);
-      // drain copies still in flight into this warp's ring, bounded
-      for (int kk = k + 1; kk < issued; ++kk)
-        if (!mbar_wait_bounded(wbar + kk % D, static_cast<uint32_t>((kk / D) & 1))) break;
-      return;
-    }
+    uint8_t* st = wsm + stage * SB;
+    // one group is committed per iteration, so the oldest D - 1 or fewer are
+    // outstanding exactly when this unit's has arrived
+    cp_async_wait<D - 1>();
+    __syncwarp();
 
     // ---- segment start: query fragments, reset state ---------------------------
     if (k == 0 || cc.p == 0) {
@@ -225,8 +340,8 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
       }
     }
 
-    const int tok0 = (cc.p + cc.off) * kFp4UnitTokens;
-    const int valid = min(kFp4UnitTokens, L - tok0);
+    const int tok0 = (cc.p + cc.off) * kUnitTokens;
+    const int valid = min(kUnitTokens, L - tok0);
     const int below = kMod ? key_low - tok0 : 0;
 
     // ---- fused append: the sequence's last unit carries the new token -------
@@ -265,8 +380,12 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
     float s[kUP][NT][4];
 #pragma unroll
     for (int u = 0; u < kUP; ++u) {
+      // two accumulators, so that an MMA does not wait for the one before it
+      float s1[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[u][nt][c] = s1[nt][c] = 0.f;
       const uint8_t* kt = st + u * kFp4TileBytes;
       // tokens g and g + 8, dims 32t .. 32t + 31
       const uint4 ka = *reinterpret_cast<const uint4*>(kt + lane * 16);
@@ -290,13 +409,17 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           mma_16816<false>(s[u][nt], xa[0], xb[0], xa[1], xb[1], qf[nt][2 * w][0], qf[nt][2 * w][1]);
-          mma_16816<false>(s[u][nt], xa[2], xb[2], xa[3], xb[3], qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+          mma_16816<false>(s1[nt], xa[2], xb[2], xa[3], xb[3], qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
         }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[u][nt][c] += s1[nt][c];
     }
 
     // ---- online softmax, one max / rescale per unit --------------------------------
-    const bool edge = valid < kFp4UnitTokens || below > 0;
+    const bool edge = valid < kUnitTokens || below > 0;
     uint32_t pb[kUP][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -399,20 +522,22 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
     __syncwarp();
 
     // ---- refill this stage with the unit D ahead -----------------------------------
-    if (issued < cnt) {
-      fence_proxy_async_smem();
-      cursor_next<kMode>(pc, p, tb, Hkv);
+    if (pc.v < end) {
       issue(stage, pc, pc.p == 0);
-      ++issued;
+      fp4_next<kMod, kUnitTokens>(pc, p, tb.prefix, end);
+    } else {
+      cp_async_commit();
     }
 
     // ---- segment end: finalize ---------------------------------------------------
-    if (cc.p == cc.P - 1 || k == cnt - 1) {
-      const int b = cc.b, h = cc.h;
-      const int64_t seg0 = static_cast<int64_t>(tb.prefix[b]) * Hkv + static_cast<int64_t>(h) * cc.P;
+    const Fp4Cursor at = cc;
+    fp4_next<kMod, kUnitTokens>(cc, p, tb.prefix, end);
+    if (at.p == at.P - 1 || cc.v >= end) {
+      const int b = at.b, h = at.h;
+      const int64_t seg0 = at.v - at.p;
       const int64_t unit = static_cast<int64_t>(b) * Hkv + h;
       const int64_t first_w = seg0 / tb.Qc;
-      const int nsplit = static_cast<int>((seg0 + cc.P - 1) / tb.Qc - first_w + 1);
+      const int nsplit = static_cast<int>((seg0 + at.P - 1) / tb.Qc - first_w + 1);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -459,47 +584,40 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
         last = __shfl_sync(0xffffffffu, last, 0);
         __syncwarp();  // lane 0's acquire orders the whole warp's reads
         if (last) {
-          combine_rows<kBF16, kRec, false>(p, first_w + unit, nsplit, -1, 0, group, b, h, 0, lane);
+          combine_split<kBF16, kRec>(p, first_w + unit, nsplit, group, b, h, lane);
           if (lane == 0) p.counters[b * Hkv + h] = 0;
         }
       }
     }
-    if (k + 1 < cnt) cursor_next<kMode>(cc, p, tb, Hkv);
   }
 }
 
 template <bool kBF16, int NT, bool kMod>
-__global__ void __launch_bounds__(kFp4Warps * 32, 1) paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
-  constexpr int D = kFp4Stages, W = kFp4Warps;
+__global__ void __launch_bounds__(fp4_warps<NT>() * 32, 1) paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
+  constexpr int D = kFp4Stages, W = fp4_warps<NT>();
+  constexpr int kUP = fp4_pages<NT>(), kUnitTokens = kUP * kPageTokens, SB = fp4_stage_bytes<NT>();
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* qslots = smem + W * D * kFp4StageBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(qslots + W * D * fp4_qslot_bytes<NT>());
-  int* prefix = reinterpret_cast<int*>(bars + W * D);
+  uint8_t* qslots = smem + W * D * SB;
+  int* prefix = reinterpret_cast<int*>(qslots + W * D * fp4_qslot_bytes<NT>());
   __shared__ int s_warp_tot[W];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int B = p.num_seqs, Hkv = p.num_kv_heads;
   const int spb = p.block_size / kPageTokens;
-  if (lane == 0) {
-    for (int s = 0; s < D; ++s) mbar_init(&bars[warp * D + s], 1);
-    fence_mbar_init();
-  }
-  // everything above overlaps the previous kernel in the stream
+  // the launch overlaps the previous kernel in the stream up to here
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   Tables tb = {};
   tb.prefix = prefix;
-  tb.mpp = tb.wp = tb.wo = 1;
-  tb.unit_tokens = kFp4UnitTokens;
 
   // ---- prologue: units per sequence and their exclusive prefix sum -------------
   const int per = (B + blockDim.x - 1) / blockDim.x;
   const int b_lo = min(B, tid * per), b_hi = min(B, b_lo + per);
   auto units_of = [&](int b) {
-    const int P = (own_pages_of(p, b, spb) + kFp4UnitPages - 1) / kFp4UnitPages;
+    const int P = (own_pages_of(p, b, spb) + kUP - 1) / kUP;
+    int real = P;
     if constexpr (kMod)
-      return P > 0 ? max(0, P - mod_first_unit(p, b, __ldg(p.seq_lens + b), kFp4UnitTokens)) : 0;
-    else
-      return P;
+      real = P > 0 ? max(0, P - mod_first_unit(p, b, __ldg(p.seq_lens + b), kUnitTokens)) : 0;
+    return real > 0 ? real + kFp4SegCost : 0;  // list positions per kv head
   };
   int bad = 0, local = 0;
   for (int b = b_lo; b < b_hi; ++b) {
@@ -540,14 +658,14 @@ __global__ void __launch_bounds__(kFp4Warps * 32, 1) paged_decode_fp4_kernel(con
   const int64_t gw = static_cast<int64_t>(blockIdx.x) * W + warp;
   const int64_t start = min(total, gw * tb.Qc), end = min(total, start + tb.Qc);
   if (start < end)
-    stream_range_fp4<kBF16, NT, kMod>(p, tb, start, end, gw, smem + warp * D * kFp4StageBytes,
-                                      qslots + warp * D * fp4_qslot_bytes<NT>(), bars + warp * D, lane);
+    stream_range_fp4<kBF16, NT, kMod>(p, tb, start, end, gw, smem + warp * D * SB,
+                                      qslots + warp * D * fp4_qslot_bytes<NT>(), lane);
 }
 
 template <bool kBF16, int NT, bool kMod>
 static int launch_fp4(const DecodeParams& p, int sm_count, cudaStream_t stream) {
   constexpr int base = fp4_smem_bytes_before_table<NT>();
-  static_assert(base + (kDecodeMaxSeqs + 1) * 4 + 1024 <= 232448, "shared memory");
+  static_assert(base + (kDecodeMaxSeqs + 1) * 4 + 256 <= 232448, "shared memory");
   static bool configured[64] = {false};  // the attribute is per function and per device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return static_cast<int>(cudaErrorInvalidDevice);
@@ -560,7 +678,7 @@ static int launch_fp4(const DecodeParams& p, int sm_count, cudaStream_t stream) 
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sm_count);
-  cfg.blockDim = dim3(kFp4Warps * 32);
+  cfg.blockDim = dim3(fp4_warps<NT>() * 32);
   cfg.dynamicSmemBytes = base + static_cast<size_t>(p.num_seqs + 1) * 4;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

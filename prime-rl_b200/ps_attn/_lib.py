@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -130,6 +131,17 @@ class PagedProblem(ctypes.Structure):
         ("k_scale", ctypes.c_void_p),
         ("v_scale", ctypes.c_void_p),
     ]
+
+
+def _struct_of(cls) -> "struct.Struct":
+    """A packer of a whole ctypes structure, in field order (native alignment)."""
+    codes = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
+    st = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_) + "0q")
+    assert st.size == ctypes.sizeof(cls)
+    return st
+
+
+PAGED_PROBLEM_STRUCT = _struct_of(PagedProblem)
 
 
 class ScoreMod(ctypes.Structure):

@@ -36,7 +36,10 @@ _DTYPES = {
 
 
 def _stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the raw handle, without the Stream object that current_stream() builds
+    # (1.5 us of a small call's host time)
+    return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None
+                                              else torch.cuda.current_device())
 
 
 def _require_cuda(*tensors):
@@ -89,7 +92,7 @@ def _check_nvfp4(key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
 def _launch(device: torch.device, fn, *args) -> None:
     """Call a C entry point with ``device`` current (the library launches on the
     current device)."""
-    if device.index is None or torch.cuda.current_device() == device.index:
+    if device.index is None or torch._C._cuda_getDevice() == device.index:
         _lib.check(fn(*args))
     else:
         with torch.cuda.device(device):
@@ -465,46 +468,28 @@ def _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
     if fp4:
         nb, hkv, bs, d = key_cache.shape[0], key_cache.shape[1], key_cache.shape[2], q.shape[-1]
     hq = q.shape[1]
-    pr = _lib.PagedProblem()
-    pr.q = q.data_ptr()
-    pr.q_stride_token, pr.q_stride_head = q.stride(0), q.stride(1)
-    pr.key_cache = key_cache.data_ptr()
-    pr.value_cache = value_cache.data_ptr()
-    pr.cache_stride_block, pr.cache_stride_slot, pr.cache_stride_head = key_cache.stride()[:3]
-    if fp4:
-        pr.cache_stride_head, pr.cache_stride_slot = key_cache.stride()[1:3]
-    pr.num_blocks = nb
-    pr.block_table = block_table.data_ptr()
-    pr.block_table_stride = block_table.stride(0)
-    pr.max_blocks_per_seq = block_table.shape[1]
-    pr.seq_lens = seq_lens.data_ptr()
-    pr.query_start_loc = query_start_loc.data_ptr() if query_start_loc is not None else None
-    pr.num_seqs = seq_lens.shape[0]
-    pr.out = out.data_ptr()
-    pr.out_stride_token, pr.out_stride_head = out.stride(0), out.stride(1)
-    if lse is not None:
-        pr.lse = lse.data_ptr()
-        pr.lse_stride_head, pr.lse_stride_token = lse.stride(0), lse.stride(1)
-    pr.num_q_heads = hq
-    pr.num_kv_heads = hkv
-    pr.head_size = d
-    pr.block_size = bs
-    pr.dtype = _DTYPES[q.dtype]
-    pr.softmax_scale = float(softmax_scale)
     if out.shape[0] < q.shape[0]:
         raise ValueError("out has fewer rows than q")
-    pr.num_tokens = q.shape[0]
-    if status is not None:
-        if status.dtype != torch.int32 or not status.is_cuda:
-            raise ValueError("status must be a CUDA int32 tensor")
-        pr.status = status.data_ptr()
-    if fp8:
-        pr.kv_cache_dtype = _lib.PS_KV_FP8_E4M3
-    elif fp4:
-        pr.kv_cache_dtype = _lib.PS_KV_NVFP4
-    pr.k_scale = _scale_ptr(k_scale)
-    pr.v_scale = _scale_ptr(v_scale)
-    return pr
+    if status is not None and (status.dtype != torch.int32 or not status.is_cuda):
+        raise ValueError("status must be a CUDA int32 tensor")
+    q_st, q_sh = q.stride()[:2]
+    o_st, o_sh = out.stride()[:2]
+    if fp4:
+        s_block, s_head, s_slot = key_cache.stride()[:3]
+    else:
+        s_block, s_slot, s_head = key_cache.stride()[:3]
+    l_sh, l_st = (lse.stride(0), lse.stride(1)) if lse is not None else (0, 0)
+    # packed in one go: setting the fields one by one costs a small call 8 us
+    return _lib.PagedProblem.from_buffer_copy(_lib.PAGED_PROBLEM_STRUCT.pack(
+        q.data_ptr(), q_st, q_sh, key_cache.data_ptr(), value_cache.data_ptr(), s_block, s_slot, s_head, nb,
+        block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
+        query_start_loc.data_ptr() if query_start_loc is not None else 0, seq_lens.shape[0],
+        out.data_ptr(), o_st, o_sh, lse.data_ptr() if lse is not None else 0, l_sh, l_st,
+        hq, hkv, d, bs, _DTYPES[q.dtype], float(softmax_scale), q.shape[0],
+        status.data_ptr() if status is not None else 0,
+        0, 0, 0, 0, 0, 0, 0,  # new_key .. slot_mapping: set by the caller
+        _lib.PS_KV_NVFP4 if fp4 else _lib.PS_KV_FP8_E4M3 if fp8 else _lib.PS_KV_AUTO,
+        _scale_ptr(k_scale) or 0, _scale_ptr(v_scale) or 0))
 
 
 def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -625,8 +610,10 @@ def dequant_gather(key_cache: torch.Tensor, value_cache: torch.Tensor, block_tab
     sequence's length are left uninitialised (never read).  Without scales
     the scratch holds the e4m3 values (nvfp4: code * block scale) exactly
     (attend over it with the scales); with them, code * scale rounded to
-    ``dtype``.  ``out``: the (key, value) scratch to write into, contiguous and
-    of that shape, instead of new tensors."""
+    ``dtype``.  ``out``: the (key, value) or (key, value, block table) of an
+    earlier call of this shape to write into instead of new tensors, contiguous;
+    the third result is then its block table (None for a pair): a caller that
+    keeps the scratch keeps the table, which does not change."""
     lib = _lib.load()
     _require_cuda(key_cache, value_cache, block_table, seq_lens)
     if not is_fp8_cache(key_cache) or value_cache.dtype != key_cache.dtype:
@@ -640,15 +627,18 @@ def dequant_gather(key_cache: torch.Tensor, value_cache: torch.Tensor, block_tab
         kd = torch.empty(B * max_pages, bs, hkv, d, dtype=dtype, device=dev)
         vd = torch.empty_like(kd)
     else:
-        kd, vd = out
+        kd, vd = out[:2]
         for x in (kd, vd):
             if tuple(x.shape) != (B * max_pages, bs, hkv, d) or x.dtype != dtype or x.device != dev \
                     or not x.is_contiguous():
                 raise ValueError(f"out must be contiguous [{B * max_pages}, {bs}, {hkv}, {d}] {dtype} on {dev}")
-    bt = torch.arange(B * max_pages, dtype=torch.int32, device=dev).view(B, max_pages)
+    if out is None:
+        bt = torch.arange(B * max_pages, dtype=torch.int32, device=dev).view(B, max_pages)
+    else:
+        bt = out[2] if len(out) > 2 else None
     if B == 0 or max_pages == 0:
         return kd, vd, bt
-    q_like = torch.empty(1, 1, d, dtype=dtype, device=dev)
+    q_like = kd.flatten(0, 1)  # (not read)
     pr = _problem(q_like, key_cache, value_cache, block_table, seq_lens, None, 1.0, q_like, None,
                   status=status, k_scale=k_scale, v_scale=v_scale)
     _launch(dev, lib.ps_kv_dequant_gather, ctypes.byref(pr), max_pages, kd.data_ptr(), vd.data_ptr(),
