@@ -55,6 +55,19 @@ __device__ __forceinline__ uint32_t hmul2_u32(uint32_t a, __half2 b) {
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t a) { return *reinterpret_cast<const __half2*>(&a); }
 
+// e2m1 codes of eight values times m, in order from the low nibble.
+__device__ __forceinline__ uint32_t e2m1x8(const float2 (&f)[4], float m) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(f[0].x * m), "f"(f[0].y * m), "f"(f[1].x * m), "f"(f[1].y * m), "f"(f[2].x * m), "f"(f[2].y * m),
+        "f"(f[3].x * m), "f"(f[3].y * m));
+  return w;
+}
+
 // Warp-collective: eight model-dtype elements of a row per lane, lanes 2i and
 // 2i + 1 holding one 16-dim block, to codes and the block's scale.
 //   scale = e4m3(max|x| / (6 g)), codes = e2m1(x / (scale * g))
@@ -63,30 +76,69 @@ __device__ __forceinline__ __half2 as_half2(uint32_t a) { return *reinterpret_ca
 // inputs land on ties of e2m1, which a rounded reciprocal would move).  A
 // block whose scale rounds to zero stores zeros; a block with a NaN stores a
 // NaN scale, so that reading it gives NaN as from a 16-bit cache.
+//
+// Only next to a tie are the divisions carried out: a product with an
+// approximate reciprocal is within 2^-21 of the quotient, so where that product
+// a little reduced and a little enlarged gives the same codes, the quotient
+// gives them too.  (With a division for each element the append was 200
+// instructions for 8 elements, and bound by them.)
+constexpr float kNearLo = 1.f - 1.f / (1 << 19), kNearHi = 1.f + 1.f / (1 << 19);
+
+template <bool kBF16>
+__device__ __forceinline__ uint32_t max2_abs_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  a &= 0x7fff7fffu;
+  b &= 0x7fff7fffu;
+  if constexpr (kBF16)
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <bool kBF16>
 __device__ __forceinline__ void quantize8_nvfp4(uint4 v, float g, uint32_t& word, uint32_t& scale) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  float2 f[4];
-  float amax = 0.f, bad = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[i] = unpack2<kBF16>(w[i]);
-    amax = fmaxf(amax, fmaxf(fabsf(f[i].x), fabsf(f[i].y)));
-    bad += (f[i].x != f[i].x || f[i].y != f[i].y) ? 1.f : 0.f;
-  }
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  bad += __shfl_xor_sync(0xffffffffu, bad, 1);
-  scale = __nv_cvt_float_to_fp8(__fdiv_rn(amax, __fmul_rn(6.f, g)), __NV_SATFINITE, __NV_E4M3);
-  if (bad > 0.f) scale = 0x7f;
+  // the block's largest magnitude, in the rows' own type (NaN if it has one)
+  uint32_t m = max2_abs_nan<kBF16>(max2_abs_nan<kBF16>(v.x, v.y), max2_abs_nan<kBF16>(v.z, v.w));
+  m = max2_abs_nan<kBF16>(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  const float2 mm = unpack2<kBF16>(m);
+  float amax;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(amax) : "f"(mm.x), "f"(mm.y));
+  const float six_g = __fmul_rn(6.f, g);
+  const bool usual = six_g > 1e-30f && six_g < 1e30f;
+  const float near = amax * rcp_approx(six_g);
+  const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(near * kNearLo, near * kNearHi), __NV_SATFINITE, __NV_E4M3);
+  scale = two & 0xffu;
+  // (below 2^-9 a flushed subnormal could hide a tie)
+  if (!usual || scale != two >> 8 || (near < 1e-30f && amax > 0.f))
+    scale = __nv_cvt_float_to_fp8(__fdiv_rn(amax, six_g), __NV_SATFINITE, __NV_E4M3);
+  if (amax != amax) scale = 0x7f;
   const __half_raw s16 = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(scale), __NV_E4M3);
   const float d = __fmul_rn(__half2float(__half(s16)), g);
   word = 0;
   if (d > 0.f) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t c = __nv_cvt_float2_to_fp4x2(make_float2(__fdiv_rn(f[i].x, d), __fdiv_rn(f[i].y, d)),
-                                                  __NV_E2M1, cudaRoundNearest);
-      word |= (c & 0xffu) << (8 * i);
+    const float2 f[4] = {unpack2<kBF16>(v.x), unpack2<kBF16>(v.y), unpack2<kBF16>(v.z), unpack2<kBF16>(v.w)};
+    uint32_t hi = 1;
+    if (d > 1e-30f && d < 1e30f) {
+      const float inv = rcp_approx(d);
+      word = e2m1x8(f, inv * kNearLo);
+      hi = e2m1x8(f, inv * kNearHi);
+    }
+    if (word != hi) {
+      word = 0;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+        const float2 x = unpack2<kBF16>(w);
+        const uint32_t c = __nv_cvt_float2_to_fp4x2(make_float2(__fdiv_rn(x.x, d), __fdiv_rn(x.y, d)), __NV_E2M1,
+                                                    cudaRoundNearest);
+        word |= (c & 0xffu) << (8 * i);
+      }
     }
   }
 }
