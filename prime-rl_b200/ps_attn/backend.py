@@ -23,6 +23,7 @@ or as an override of FLASH_ATTN::
     register()                      # CUSTOM
     register(override_flash=True)   # FLASH_ATTN -> PS
     register(rope_fusion=True)      # variant with the fused RoPE + KV append
+    register(score_mods=True)       # variant with ALiBi, sliding window and soft-cap
 
 The ``rope_fusion`` variant (:class:`PSRopeAttentionBackend`) keeps
 FlashAttention's ``forward_includes_kv_cache_update = False``, so vLLM issues
@@ -45,13 +46,22 @@ append (bit-identical to ``reshape_and_cache_flash`` with "fp8") and read by
 the decode kernel's fp8 mode; prefill requests attend over their pages
 copied into a 16-bit scratch (``ops.dequant_gather``: the e4m3 values are
 exact in bf16) and attended with the scales applied in the prefill kernel.
-Unsupported options (ALiBi, sliding window, soft-cap, sinks, other KV-cache
-dtypes, encoder attention) raise ``NotImplementedError`` at construction.
+A 4-bit KV cache (``kv_cache_dtype`` "nvfp4") takes the 72 bytes per token and
+head that vLLM budgets for it (``vllm/utils/torch_utils.py:415-417``), in this
+backend's own order (``ops.nvfp4_cache_shape``), under the same per-tensor
+scales: the decode's append is fused, prefill requests attend over their pages
+gathered into the 16-bit scratch.
+The ``score_mods`` variant (:class:`PSScoreModAttentionBackend`) takes vLLM's
+``alibi_slopes``, ``sliding_window`` and ``logits_soft_cap``, which the plain
+backend refuses; it does not use shared-prefix plans.
+Unsupported options (sinks, other KV-cache dtypes, encoder attention; in the
+plain backend ALiBi, sliding window and soft-cap) raise ``NotImplementedError``
+at construction.
 """
 from __future__ import annotations
 
 import os
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import ClassVar
 
 import torch
@@ -68,7 +78,8 @@ BACKEND_NAME = "CUSTOM"
 
 class PSAttentionBackend(AttentionBackend):
     supported_dtypes: ClassVar[list[torch.dtype]] = [torch.float16, torch.bfloat16]
-    supported_kv_cache_dtypes: ClassVar[list[str]] = ["auto", "float16", "bfloat16", "fp8", "fp8_e4m3"]
+    supported_kv_cache_dtypes: ClassVar[list[str]] = ["auto", "float16", "bfloat16", "fp8", "fp8_e4m3",
+                                                       "nvfp4"]
     forward_includes_kv_cache_update: bool = True
 
     @staticmethod
@@ -92,6 +103,8 @@ class PSAttentionBackend(AttentionBackend):
                            cache_dtype_str: str = "auto") -> tuple[int, ...]:
         if block_size % 16 != 0:
             raise ValueError("Block size must be a multiple of 16.")
+        if cache_dtype_str == "nvfp4":
+            return (2, *ops.nvfp4_cache_shape(num_blocks, block_size, num_kv_heads, head_size))
         return (2, num_blocks, block_size, num_kv_heads, head_size)
 
     @staticmethod
@@ -220,6 +233,8 @@ class PSAttentionImpl(AttentionImpl):
     # forward appends the step's keys and values (the backend declares
     # forward_includes_kv_cache_update = True)
     appends_in_forward: bool = True
+    # ALiBi, sliding window and soft-cap (PSScoreModAttentionImpl)
+    takes_score_mods: bool = False
 
     def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int,
                  alibi_slopes: list[float] | None, sliding_window: int | None,
@@ -227,15 +242,15 @@ class PSAttentionImpl(AttentionImpl):
                  attn_type: str = AttentionType.DECODER,
                  kv_sharing_target_layer_name: str | None = None,
                  sinks: torch.Tensor | None = None) -> None:
-        if alibi_slopes is not None:
+        if alibi_slopes is not None and not self.takes_score_mods:
             raise NotImplementedError("ALiBi is not supported by the PS backend")
-        if sliding_window is not None:
+        if sliding_window is not None and not self.takes_score_mods:
             raise NotImplementedError("sliding window is not supported by the PS backend")
-        if logits_soft_cap:
+        if logits_soft_cap and not self.takes_score_mods:
             raise NotImplementedError("logits soft-cap is not supported by the PS backend")
         if sinks is not None:
             raise NotImplementedError("attention sinks are not supported by the PS backend")
-        if kv_cache_dtype not in ("auto", "float16", "bfloat16", "fp8", "fp8_e4m3"):
+        if kv_cache_dtype not in ("auto", "float16", "bfloat16", "fp8", "fp8_e4m3", "nvfp4"):
             raise NotImplementedError(f"kv_cache_dtype {kv_cache_dtype} not supported")
         if attn_type != AttentionType.DECODER:
             raise NotImplementedError("the PS backend implements decoder attention only")
@@ -248,23 +263,30 @@ class PSAttentionImpl(AttentionImpl):
         # by the metadata builder).
         self.dcp = getattr(self, "dcp_world_size", 1) > 1
         if self.dcp and kv_cache_dtype not in ("auto", "float16", "bfloat16"):
-            raise NotImplementedError("decode context parallelism over an fp8 cache is not supported")
+            raise NotImplementedError(f"decode context parallelism over an {kv_cache_dtype} cache is not supported")
         self.num_heads = num_heads
         self.head_size = head_size
         self.scale = float(scale)
         self.num_kv_heads = num_kv_heads
         self.kv_cache_dtype = kv_cache_dtype
         self.fp8 = kv_cache_dtype in ("fp8", "fp8_e4m3")
+        self.nvfp4 = kv_cache_dtype == "nvfp4"
+        self.quantized = self.fp8 or self.nvfp4
+        self._score_mod = None
         self.kv_sharing_target_layer_name = kv_sharing_target_layer_name
         self.attn_type = attn_type
         self.num_queries_per_kv = num_heads // num_kv_heads
 
     def _scales(self, layer) -> dict:
-        """The layer's fp8 dequantization scales (vLLM's ``_k_scale`` /
+        """The layer's fp8 / nvfp4 dequantization scales (vLLM's ``_k_scale`` /
         ``_v_scale``), none for a 16-bit cache."""
-        if not self.fp8:
+        if not self.quantized:
             return {}
         return dict(k_scale=getattr(layer, "_k_scale", None), v_scale=getattr(layer, "_v_scale", None))
+
+    def score_mod(self, device) -> "ops.ScoreMod | None":
+        """The layer's score modifiers (none in the plain backend)."""
+        return self._score_mod
 
     def do_kv_cache_update(self, layer, key: torch.Tensor, value: torch.Tensor,
                            kv_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
@@ -289,6 +311,7 @@ class PSAttentionImpl(AttentionImpl):
         append = (self.appends_in_forward and key is not None and value is not None
                   and self.kv_sharing_target_layer_name is None)
         sc = self._scales(layer)
+        mod = self.score_mod(query.device)
         if append and T > ndt:  # prefill tokens: into the cache before their attention
             ops.kv_append(key[ndt:T], value[ndt:T], key_cache, value_cache, m.slot_mapping[ndt:T], **sc)
         if nd > 0:
@@ -296,19 +319,20 @@ class PSAttentionImpl(AttentionImpl):
             ops.paged_decode(query[:ndt], key_cache, value_cache, m.block_table[:nd],
                              m.seq_lens[:nd], self.scale, output[:ndt],
                              query_start_loc=m.query_start_loc[:nd + 1], workspace=m.workspace,
-                             cascade=None if self.fp8 else m.cascade_plan, **fused, **sc)
+                             cascade=None if self.quantized or mod is not None else m.cascade_plan,
+                             score_mod=mod, **fused, **sc)
         if m.num_prefills > 0:
             kc, vc, bt = key_cache, value_cache, m.block_table[nd:]
-            if self.fp8:
-                # the prefill kernel reads 16-bit pages: the e4m3 values
-                # exactly (unscaled), with the scales applied in the kernel
-                bs = key_cache.shape[1]
+            if self.quantized:
+                # the prefill kernel reads 16-bit pages: the e4m3 (e2m1 * block
+                # scale) values exactly, unscaled, with the tensors' scales
+                # applied in the kernel
+                bs = key_cache.shape[2] if self.nvfp4 else key_cache.shape[1]
                 kc, vc, bt = ops.dequant_gather(key_cache, value_cache, bt, m.seq_lens[nd:],
                                                 (m.max_seq_len + bs - 1) // bs, query.dtype)
             ops.chunked_prefill(query[:T], kc, vc, bt, m.seq_lens[nd:], m.query_start_loc[nd:],
-                                self.scale, output[:T], workspace=m.workspace, **sc)
+                                self.scale, output[:T], workspace=m.workspace, score_mod=mod, **sc)
         return output
-
 
     def _forward_dcp(self, query, key, value, key_cache, value_cache, m, output):
         """Decode context parallelism (``flash_attn.py:885-983``): the cache
@@ -340,9 +364,9 @@ class PSRopeAttentionImpl(PSAttentionImpl):
     appends_in_forward: bool = False
 
     def fused_rope_kvcache_supported(self) -> bool:
-        # the fused kernel stores 16-bit rows; an fp8 cache takes the plain
+        # the fused kernel stores 16-bit rows; a quantized cache takes the plain
         # (quantizing) KV update instead
-        return not self.fp8
+        return not self.quantized
 
     def do_rope_and_kv_cache_update(self, layer, query: torch.Tensor, key: torch.Tensor,
                                     value: torch.Tensor, positions: torch.Tensor,
@@ -364,16 +388,61 @@ class PSRopeAttentionBackend(PSAttentionBackend):
         return PSRopeAttentionImpl
 
 
+class PSScoreModAttentionImpl(PSAttentionImpl):
+    """Impl for :class:`PSScoreModAttentionBackend`: FlashAttention's
+    ``alibi_slopes``, ``sliding_window`` and ``logits_soft_cap``
+    (``flash_attn.py:595-640``: a window of W tokens is the row's own and the
+    W - 1 before it)."""
+
+    takes_score_mods: bool = True
+
+    def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int,
+                 alibi_slopes: list[float] | None = None, sliding_window: int | None = None,
+                 kv_cache_dtype: str = "auto", logits_soft_cap: float | None = None, **kwargs) -> None:
+        super().__init__(num_heads, head_size, scale, num_kv_heads, alibi_slopes, sliding_window,
+                         kv_cache_dtype, logits_soft_cap, **kwargs)
+        if self.dcp:
+            raise NotImplementedError("decode context parallelism with score modifiers is not supported")
+        if sliding_window is not None and sliding_window < 1:
+            raise ValueError(f"sliding_window {sliding_window} must be at least 1")
+        slopes = None
+        if alibi_slopes is not None:
+            slopes = torch.tensor(alibi_slopes, dtype=torch.float32)
+            if slopes.shape != (num_heads,):
+                raise ValueError(f"{slopes.numel()} ALiBi slopes for {num_heads} heads")
+        if slopes is not None or sliding_window is not None or logits_soft_cap:
+            self._score_mod = ops.ScoreMod(
+                softcap=float(logits_soft_cap or 0.0), alibi_slopes=slopes,
+                window_left=-1 if sliding_window is None else sliding_window - 1)
+
+    def score_mod(self, device) -> "ops.ScoreMod | None":
+        m = self._score_mod
+        if m is not None and m.alibi_slopes is not None and m.alibi_slopes.device != device:
+            # once, in the first eager step (before any graph capture)
+            m = self._score_mod = replace(m, alibi_slopes=m.alibi_slopes.to(device))
+        return m
+
+
+class PSScoreModAttentionBackend(PSAttentionBackend):
+    @staticmethod
+    def get_impl_cls() -> type["PSScoreModAttentionImpl"]:
+        return PSScoreModAttentionImpl
+
+
 def cascade_enabled() -> bool:
     """Shared-prefix decode is opt-in (``PS_ATTN_CASCADE=1``)."""
     return os.environ.get("PS_ATTN_CASCADE", "0") == "1"
 
 
-def register(override_flash: bool = False, rope_fusion: bool = False) -> None:
+def register(override_flash: bool = False, rope_fusion: bool = False, score_mods: bool = False) -> None:
     """Register the PS backend with vLLM's backend registry (``rope_fusion``:
-    the variant whose KV update vLLM issues, fusable with RoPE)."""
+    the variant whose KV update vLLM issues, fusable with RoPE; ``score_mods``:
+    the variant with ALiBi, sliding window and soft-cap)."""
+    if rope_fusion and score_mods:
+        raise ValueError("rope_fusion and score_mods are separate variants")
     from vllm.v1.attention.backends.registry import AttentionBackendEnum, register_backend
 
-    cls = PSRopeAttentionBackend if rope_fusion else PSAttentionBackend
+    cls = (PSRopeAttentionBackend if rope_fusion else PSScoreModAttentionBackend if score_mods
+           else PSAttentionBackend)
     target = AttentionBackendEnum.FLASH_ATTN if override_flash else AttentionBackendEnum.CUSTOM
     register_backend(target, f"{cls.__module__}.{cls.__qualname__}")
