@@ -112,9 +112,10 @@ __device__ __forceinline__ void fp4_next(Fp4Cursor& c, const DecodeParams& p, co
   fp4_sequence<kMod, kUnitTokens>(c, p, prefix);
 }
 
-// First unit at or after position v; v < end <= the list's length.
+// The segment that position v lies in and v's place there, which may be one of
+// its empty positions (p >= P).
 template <bool kMod, int kUnitTokens>
-__device__ __forceinline__ Fp4Cursor fp4_seek(int64_t v, int64_t end, const DecodeParams& p, const int* prefix) {
+__device__ __forceinline__ Fp4Cursor fp4_locate(int64_t v, const DecodeParams& p, const int* prefix) {
   Fp4Cursor c;
   int lo = 0, hi = p.num_seqs - 1;  // largest b with prefix[b] * Hkv <= v
   while (lo < hi) {
@@ -131,12 +132,26 @@ __device__ __forceinline__ Fp4Cursor fp4_seek(int64_t v, int64_t end, const Deco
   c.h = static_cast<int>(r / V);
   c.p = static_cast<int>(r - static_cast<int64_t>(c.h) * V);
   fp4_sequence<kMod, kUnitTokens>(c, p, prefix);
+  return c;
+}
+
+// First unit at or after position v; v < end <= the list's length.
+template <bool kMod, int kUnitTokens>
+__device__ __forceinline__ Fp4Cursor fp4_seek(int64_t v, int64_t end, const DecodeParams& p, const int* prefix) {
+  Fp4Cursor c = fp4_locate<kMod, kUnitTokens>(v, p, prefix);
   if (c.p >= c.P) {  // an empty position: the next segment's first unit
     --c.v;
     --c.p;
     fp4_next<kMod, kUnitTokens>(c, p, prefix, end);
   }
   return c;
+}
+
+__device__ __forceinline__ SplitSeg fp4_split(const Fp4Cursor& c, int num_kv_heads, int64_t Qc) {
+  const int64_t seg0 = c.v - c.p;
+  SplitSeg g = {c.b, c.h, static_cast<int64_t>(c.b) * num_kv_heads + c.h, seg0 / Qc, 0};
+  g.nsplit = static_cast<int>((seg0 + c.P - 1) / Qc - g.first_w + 1);
+  return g;
 }
 
 // One warp streams the units of list positions [start, end).
@@ -260,6 +275,7 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
   float sc[NT][2];     // score scale of this lane's head columns (exp2 domain)
   float slope[NT][2];  // score modifiers: bias slopes (times log2 e)
   int L = 0, key_low = 0, cseg = 0;
+  int pending = 0;  // merges this warp owes: 1 its first segment's, 2 its last one's
   const bool fused = p.new_key != nullptr;
   uint4 new_row = make_uint4(0u, 0u, 0u, 0u);
   int64_t new_slot = -1;
@@ -534,10 +550,8 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
     fp4_next<kMod, kUnitTokens>(cc, p, tb.prefix, end);
     if (at.p == at.P - 1 || cc.v >= end) {
       const int b = at.b, h = at.h;
-      const int64_t seg0 = at.v - at.p;
-      const int64_t unit = static_cast<int64_t>(b) * Hkv + h;
-      const int64_t first_w = seg0 / tb.Qc;
-      const int nsplit = static_cast<int>((seg0 + at.P - 1) / tb.Qc - first_w + 1);
+      const SplitSeg sg = fp4_split(at, Hkv, tb.Qc);
+      const int nsplit = sg.nsplit;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -562,7 +576,7 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
             }
             if (g == 0 && p.lse) p.lse[qh * p.lse_sh + qrow * p.lse_st] = lse;
           } else {
-            const int64_t slot = gw + unit;
+            const int64_t slot = gw + sg.unit;
             float4* po = reinterpret_cast<float4*>(slot_o<kRec>(p, slot, col) + 8 * g);
 #pragma unroll
             for (int mq = 0; mq < 2; ++mq)
@@ -573,23 +587,14 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
             if (g == 0) *slot_lse<kRec>(p, slot, col) = lse;
           }
         }
-      if (nsplit > 1) {
-        // release: the warp's partial is visible (gpu scope) before the count
-        __syncwarp();
-        int last = 0;
-        if (lane == 0) {
-          last = atomic_add_release_gpu(p.counters + b * Hkv + h, 1) == nsplit - 1;
-          if (last) fence_acq_rel_gpu();  // acquire the other splits' partials
-        }
-        last = __shfl_sync(0xffffffffu, last, 0);
-        __syncwarp();  // lane 0's acquire orders the whole warp's reads
-        if (last) {
-          combine_split<kBF16, kRec>(p, first_w + unit, nsplit, group, b, h, lane);
-          if (lane == 0) p.counters[b * Hkv + h] = 0;
-        }
-      }
+      if (nsplit > 1 && count_record(p, sg, gw, lane)) pending |= at.v - at.p < start ? 1 : 2;
     }
   }
+  for (int i = 1; i <= 2; ++i)
+    if (pending & i) {
+      const Fp4Cursor c = fp4_locate<kMod, kUnitTokens>(i == 1 ? start : end - 1, p, tb.prefix);
+      merge_split<kBF16, kRec>(p, fp4_split(c, Hkv, tb.Qc), gw, lane);
+    }
 }
 
 template <bool kBF16, int NT, bool kMod>

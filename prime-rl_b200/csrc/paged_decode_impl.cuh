@@ -510,84 +510,182 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // The same merge for the kernels without a prefix segment (score modifiers,
-// 4-bit caches): slots [slot0, slot0 + n), rows [0, nrows), to out / lse.  The
-// partial rows are loaded 16 at a time (two rows of eight sources) before any
-// of them is used, so a merge waits for L2 once per 16 rows instead of once per
-// source: merging 24 sources of 2 rows went from 19,000 cycles, over half of a
-// one-sequence call (18.3 us), to under 4,000 (12.5 us).  A version that takes eight
-// rows at once waits less but is four times the code, and code that runs once
-// per segment comes from L2: 13.2 us.  More than 32 sources are folded in with a
-// running maximum.
-template <bool kBF16, int kRec>
-__device__ __noinline__ void combine_split(const DecodeParams& p, int64_t slot0, int n, int nrows, int b, int h,
-                                           int lane) {
-  constexpr int R = 2, S = 8;
+// 4-bit caches): n sources, slots slot0 + k * stride, rows j0 .. of each (at most
+// NR), to out / lse; kToRecord: into slot0's record (every read of a row precedes
+// its write).  The weights of all rows are found together, and partial rows are
+// loaded 16 or 32 at a time (all rows of S sources) before any is used, so
+// that a merge waits for L2 once per batch instead of once per source: merging
+// 24 sources of 2 rows in a loop over the sources took 19,000 cycles, over half of
+// a one-sequence call.  The loops stay rolled: code that runs once per segment is
+// fetched from L2.  More than 32 sources are folded in with a running maximum.
+template <bool kBF16, int kRec, bool kToRecord, int NR>
+__device__ __noinline__ void combine_split_rows(const DecodeParams& p, int64_t slot0, int n, int stride, int j0,
+                                                int nrows, int b, int h, int lane) {
+  constexpr int S = 16 / NR;
   constexpr float kLog2e = 1.4426950408889634f;
-  const int64_t qrow = p.qsl ? __ldg(p.qsl + b) : b;
-  for (int j0 = 0; j0 < nrows; j0 += R) {
-    float4 acc[R];
-    float mrun[R], sum[R];
+  float4 acc[NR];
+  float mrun[NR], sum[NR];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-      mrun[r] = -INFINITY;
-      sum[r] = 0.f;
-    }
-    for (int k0 = 0; k0 < n; k0 += 32) {
-      const int kn = min(32, n - k0);
-      float w[R];  // lane k: weight of source k0 + k
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        w[r] = lane < kn && j0 + r < nrows ? __ldcg(slot_lse<kRec>(p, slot0 + k0 + lane, j0 + r)) : -INFINITY;
+  for (int r = 0; r < NR; ++r) {
+    acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    mrun[r] = -INFINITY;
+    sum[r] = 0.f;
+  }
 #pragma unroll 1
-      for (int s0 = 0; s0 < kn; s0 += S) {
-        float4 v[R][S];
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    const int kn = min(32, n - k0);
+    float w[NR];  // lane k: weight of source k0 + k
 #pragma unroll
-        for (int i = 0; i < S; ++i)
+    for (int r = 0; r < NR; ++r)
+      w[r] = lane < kn && r < nrows ? __ldcg(slot_lse<kRec>(p, slot0 + (k0 + lane) * stride, j0 + r)) : -INFINITY;
+#pragma unroll 1
+    for (int s0 = 0; s0 < kn; s0 += S) {
+      float4 v[S][NR];
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-            v[r][i] = s0 + i < kn && j0 + r < nrows
-                          ? __ldcg(reinterpret_cast<const float4*>(slot_o<kRec>(p, slot0 + k0 + s0 + i, j0 + r)) + lane)
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
-        if (s0 == 0) {  // the chunk's weights, while the rows are on their way
+      for (int i = 0; i < S; ++i)
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float mx = fmaxf(mrun[r], warp_max(w[r]));
-            const float ref = mx == -INFINITY ? 0.f : mx;
-            const float alpha = ex2((mrun[r] - ref) * kLog2e);
-            w[r] = ex2((w[r] - ref) * kLog2e);  // empty sources: 0
-            sum[r] = sum[r] * alpha + warp_sum(w[r]);
-            acc[r].x *= alpha;
-            acc[r].y *= alpha;
-            acc[r].z *= alpha;
-            acc[r].w *= alpha;
-            mrun[r] = mx;
-          }
+        for (int r = 0; r < NR; ++r)
+          v[i][r] = s0 + i < kn && r < nrows
+                        ? __ldcg(reinterpret_cast<const float4*>(
+                                     slot_o<kRec>(p, slot0 + (k0 + s0 + i) * stride, j0 + r)) + lane)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 == 0) {  // the chunk's weights, while the rows are on their way
+        float mx[NR], sm[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) mx[r] = w[r];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int r = 0; r < NR; ++r) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], o));
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          mx[r] = fmaxf(mx[r], mrun[r]);
+          const float ref = mx[r] == -INFINITY ? 0.f : mx[r];
+          const float alpha = ex2((mrun[r] - ref) * kLog2e);
+          w[r] = ex2((w[r] - ref) * kLog2e);  // empty sources: 0
+          sm[r] = w[r];
+          sum[r] *= alpha;
+          acc[r].x *= alpha;
+          acc[r].y *= alpha;
+          acc[r].z *= alpha;
+          acc[r].w *= alpha;
+          mrun[r] = mx[r];
         }
 #pragma unroll
-        for (int i = 0; i < S; ++i)
+        for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float wk = __shfl_sync(0xffffffffu, w[r], s0 + i);  // 0 past kn
-            acc[r].x += wk * v[r][i].x;
-            acc[r].y += wk * v[r][i].y;
-            acc[r].z += wk * v[r][i].z;
-            acc[r].w += wk * v[r][i].w;
-          }
+          for (int r = 0; r < NR; ++r) sm[r] += __shfl_xor_sync(0xffffffffu, sm[r], o);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) sum[r] += sm[r];
       }
-    }
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (j0 + r >= nrows) break;
-      const float inv = (sum[r] == 0.f || sum[r] != sum[r]) ? 0.f : 1.f / sum[r];
+      for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float wk = __shfl_sync(0xffffffffu, w[r], (s0 + i) & 31);
+          if (s0 + i < kn) {
+            acc[r].x += wk * v[i][r].x;
+            acc[r].y += wk * v[i][r].y;
+            acc[r].z += wk * v[i][r].z;
+            acc[r].w += wk * v[i][r].w;
+          }
+        }
+    }
+  }
+  const int64_t qrow = p.qsl ? __ldg(p.qsl + b) : b;
+  if constexpr (kToRecord) __syncwarp();
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    if (r >= nrows) break;
+    const float inv = (sum[r] == 0.f || sum[r] != sum[r]) ? 0.f : 1.f / sum[r];
+    const float lse = __logf(sum[r]) + mrun[r];
+    if constexpr (kToRecord) {
+      reinterpret_cast<float4*>(slot_o<kRec>(p, slot0, j0 + r))[lane] =
+          make_float4(acc[r].x * inv, acc[r].y * inv, acc[r].z * inv, acc[r].w * inv);
+      if (lane == 0) *slot_lse<kRec>(p, slot0, j0 + r) = lse;
+    } else {
       const int qh = h * p.group + j0 + r;
       uint2 packed;
       packed.x = pack2<kBF16>(acc[r].x * inv, acc[r].y * inv);
       packed.y = pack2<kBF16>(acc[r].z * inv, acc[r].w * inv);
       *reinterpret_cast<uint2*>(static_cast<char*>(p.out) + (qrow * p.o_st + qh * p.o_sh + lane * 4) * 2) = packed;
-      if (lane == 0 && p.lse != nullptr) p.lse[qh * p.lse_sh + qrow * p.lse_st] = __logf(sum[r]) + mrun[r];
+      if (lane == 0 && p.lse != nullptr) p.lse[qh * p.lse_sh + qrow * p.lse_st] = lse;
     }
   }
+}
+template <bool kBF16, int kRec, bool kToRecord>
+__device__ __forceinline__ void combine_split(const DecodeParams& p, int64_t slot0, int n, int stride, int nrows,
+                                              int b, int h, int lane) {
+  if (nrows <= 2) {
+    combine_split_rows<kBF16, kRec, kToRecord, 2>(p, slot0, n, stride, 0, nrows, b, h, lane);
+  } else {
+    for (int j0 = 0; j0 < nrows; j0 += 8)
+      combine_split_rows<kBF16, kRec, kToRecord, 8>(p, slot0, n, stride, j0, min(8, nrows - j0), b, h, lane);
+  }
+}
+
+// Count one contribution into *counter; true (for the whole warp) for the last
+// of `total`, whose later reads then see every contribution.
+__device__ __forceinline__ bool count_split(int32_t* counter, int total, int lane) {
+  __syncwarp();  // release: the warp's writes are visible (gpu scope) before the count
+  int last = 0;
+  if (lane == 0) {
+    last = atomic_add_release_gpu(counter, 1) == total - 1;
+    if (last) fence_acq_rel_gpu();
+  }
+  last = __shfl_sync(0xffffffffu, last, 0);
+  __syncwarp();  // lane 0's acquire orders the whole warp's reads
+  return last != 0;
+}
+
+// Merging a segment that warps [first_w, first_w + nsplit) share, each of them
+// having written its record and counted it (count_record): the warp that was
+// last merges (merge_split).  Many splits (a long sequence with few others beside
+// it) are merged in two levels -- the last warp of each chunk of 16 or 32 splits
+// merges the chunk into its first record, the last chunk to be done merges the
+// chunks.  One sequence of 32,768 tokens, 8 / 1 heads, 4-bit (512 splits): 255 us
+// with one level, 33 with two.  (Chunk counters: pre_counters, free without a
+// cascade plan.  Two segments of more than 32 splits can share a warp only as
+// one's last and the other's first, hence two counters per warp.)
+//
+// A warp streams a contiguous range, so only the first and the last segment of
+// its range can be shared.  Its merges wait until the range is done: inside the
+// streaming loop, a merge's registers became the loop's spills (64 sequences of
+// 1k-4k: 49 us, and 103 with the merge below).
+struct SplitSeg {
+  int b, h;
+  int64_t unit, first_w;  // unit = b * Hkv + h
+  int nsplit;
+};
+__device__ __forceinline__ int split_chunk(int nsplit) { return nsplit <= 32 ? nsplit : nsplit <= 256 ? 16 : 32; }
+
+__device__ __forceinline__ int32_t* chunk_counter(const DecodeParams& p, const SplitSeg& g, int chunk) {
+  if (g.nsplit <= 32) return p.counters + g.unit;
+  return p.pre_counters + 2 * (g.first_w + chunk * split_chunk(g.nsplit)) + (chunk > 0 ? 1 : 0);
+}
+
+// True for the whole warp if its record was its chunk's last.
+__device__ __forceinline__ bool count_record(const DecodeParams& p, const SplitSeg& g, int64_t gw, int lane) {
+  const int size = split_chunk(g.nsplit), chunk = static_cast<int>(gw - g.first_w) / size;
+  return count_split(chunk_counter(p, g, chunk), min(size, g.nsplit - chunk * size), lane);
+}
+
+template <bool kBF16, int kRec>
+__device__ __forceinline__ void merge_split(const DecodeParams& p, const SplitSeg& g, int64_t gw, int lane) {
+  const int64_t slot0 = g.first_w + g.unit;
+  int32_t* counter = p.counters + g.unit;
+  const int size = split_chunk(g.nsplit);
+  const int chunks = (g.nsplit + size - 1) / size;
+  if (chunks > 1) {
+    const int chunk = static_cast<int>(gw - g.first_w) / size, members = min(size, g.nsplit - chunk * size);
+    if (lane == 0) *chunk_counter(p, g, chunk) = 0;
+    if (members > 1)
+      combine_split<kBF16, kRec, true>(p, slot0 + chunk * size, members, 1, p.group, g.b, g.h, lane);
+    if (!count_split(counter, chunks, lane)) return;
+  }
+  combine_split<kBF16, kRec, false>(p, slot0, chunks > 1 ? chunks : g.nsplit, chunks > 1 ? size : 1, p.group, g.b,
+                                    g.h, lane);
+  if (lane == 0) *counter = 0;
 }
 
 template <int NT>
@@ -857,6 +955,7 @@ __device__ __forceinline__ int stream_range(const DecodeParams& p, const CUtenso
   // score modifiers: this row's first visible key, and the bias slopes (times
   // log2 e) of this lane's head columns
   int key_low = 0;
+  int pending = 0;  // merges this warp owes: 1 its first segment's, 2 its last one's
   float slope[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) slope[nt][0] = slope[nt][1] = 0.f;
@@ -1293,6 +1392,10 @@ __device__ __forceinline__ int stream_range(const DecodeParams& p, const CUtenso
             }
           }
         } else {
+          if constexpr (kMode == kModded) {
+            const SplitSeg sg = {b, h, unit, first_w, nsplit};
+            if (count_record(p, sg, gw, lane)) pending |= seg0 < start ? 1 : 2;
+          } else {
           const int total = nsplit + (member ? 1 : 0);
           int last = 0;
           if (lane == 0) {
@@ -1306,17 +1409,25 @@ __device__ __forceinline__ int stream_range(const DecodeParams& p, const CUtenso
             int64_t xslot = -1;
             int xrow0 = 0;
             if (member) prefix_result(p, tb, __ldg(p.cas_seq_group + b), b, h, Hkv, xslot, xrow0);
-            if constexpr (kMode == kModded)
-              combine_split<kBF16, kRec>(p, first_w + unit, nsplit, group, b, h, lane);
-            else
-              combine_rows<kBF16, kRec, false>(p, first_w + unit, nsplit, xslot, xrow0, group, b, h, 0,
-                                               lane);
+            combine_rows<kBF16, kRec, false>(p, first_w + unit, nsplit, xslot, xrow0, group, b, h, 0,
+                                             lane);
             if (lane == 0) p.counters[b * Hkv + h] = 0;
+          }
           }
         }
       }
     }
     if (k + 1 < cnt) cursor_next<kMode>(cc, p, tb, Hkv);
+  }
+  if constexpr (kMode == kModded) {
+    for (int i = 1; i <= 2; ++i) {
+      if (!(pending & i)) continue;
+      const Cursor c = cursor_at<kMode>(i == 1 ? start : end - 1, p, tb, Hkv);
+      const int64_t seg0 = static_cast<int64_t>(tb.prefix[c.b]) * Hkv + static_cast<int64_t>(c.h) * c.P;
+      SplitSeg sg = {c.b, c.h, static_cast<int64_t>(c.b) * Hkv + c.h, seg0 / tb.Qc, 0};
+      sg.nsplit = static_cast<int>((seg0 + c.P - 1) / tb.Qc - sg.first_w + 1);
+      merge_split<kBF16, kRec>(p, sg, gw, lane);
+    }
   }
   return k0 + cnt;
 }
