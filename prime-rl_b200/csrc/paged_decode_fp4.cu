@@ -41,6 +41,18 @@ template <int NT>
 __host__ __device__ constexpr int fp4_warps() {
   return NT == 1 ? kDecodeFp4Warps : kDecodeFp4Warps2;
 }
+// Four more warps copy for the streaming warps, two each.  Copying is addresses and
+// shuffles with little to overlap them, 1,000 of the 4,400 cycles a unit took a
+// warp that did both.  Registers: 384 threads start with 168 each; the
+// streaming warps take the copying warps' share (256 * 216 + 128 * 72 = 384 * 168).
+constexpr int kFp4Feeds = 2;
+constexpr int kFp4StreamRegs = 216, kFp4CopyRegs = 72;
+template <int NT>
+__host__ __device__ constexpr int fp4_threads() {
+  static_assert(fp4_warps<NT>() == 8, "two warpgroups of streaming warps, one of copying warps");
+  static_assert(256 * kFp4StreamRegs + 128 * kFp4CopyRegs <= 384 * 168, "the launch's registers");
+  return (fp4_warps<NT>() + 4) * 32;
+}
 template <int NT>
 __host__ __device__ constexpr int fp4_stage_bytes() {  // K tiles, then V tiles
   return 2 * fp4_pages<NT>() * kFp4TileBytes;
@@ -56,10 +68,20 @@ __device__ __forceinline__ void cp_async16(uint32_t smem_dst, const void* gsrc) 
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(gsrc))
                : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+// This thread's arrival on `bar`, once its asynchronous copies so far are done.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // Query slot: unpadded rows (they are read once per segment, and the padding
@@ -71,8 +93,8 @@ __host__ __device__ constexpr int fp4_qslot_bytes() {
 }
 template <int NT>
 __host__ __device__ constexpr int fp4_smem_bytes_before_table() {
-  // stages | per-warp query slots
-  return fp4_warps<NT>() * kFp4Stages * (fp4_stage_bytes<NT>() + fp4_qslot_bytes<NT>());
+  // stages | per-warp query slots | full and empty barriers
+  return fp4_warps<NT>() * kFp4Stages * (fp4_stage_bytes<NT>() + fp4_qslot_bytes<NT>() + 16);
 }
 
 // Position in the list.  A segment (sequence, kv head) of P units takes P +
@@ -154,119 +176,174 @@ __device__ __forceinline__ SplitSeg fp4_split(const Fp4Cursor& c, int num_kv_hea
   return g;
 }
 
-// One warp streams the units of list positions [start, end).
+// The copying side of one streaming warp (kept by a copying warp).  Its list
+// positions are [pc.v, end).
+struct Fp4Feed {
+  Fp4Cursor pc;  // next unit to copy
+  int64_t end;
+  int k;         // units copied so far
+  int pseg;      // segments started so far
+  // Block-table entries are held 64 at a time, [bt_e0, bt_e0 + 64) of sequence
+  // bt_b: the second half is loaded when the first comes into use, so that
+  // only a new sequence waits for its entries.
+  int bt_b, bt_e0, bt_reg, bt_next;
+};
+
+// Copy the next unit into its stage: two 512-byte warp copies of codes per tile,
+// and one warp copy for the scale rows (128 bytes) of four tiles.  Pages past the
+// sequence or below the visible range are neither copied nor looked up (their
+// tokens are masked).  (Bulk copies, one per tile, cost 140 cycles each to
+// issue: their operands are uniform, so lanes take turns.)
+template <int NT, bool kMod>
+__device__ __forceinline__ void fp4_copy_unit(Fp4Feed& f, const DecodeParams& p, uint8_t* wsm, uint8_t* wq,
+                                              uint64_t* full, const int* prefix, uint64_t spb_inv, uint64_t kv_policy,
+                                              int lane) {
+  constexpr int D = kFp4Stages;
+  constexpr int kUP = fp4_pages<NT>();
+  constexpr int SB = fp4_stage_bytes<NT>();
+  static_assert(kUP % 2 == 0 && kUP <= 32, "the scale rows of a unit are copied four tiles at a time");
+  static_assert(SB % 128 == 0, "stage alignment");
+  const Fp4Cursor& c = f.pc;
+  const int spb = p.block_size / kPageTokens;
+  const int stage = f.k % D;
+  // page / spb without a division: spb is in [1, 16] and a page index below
+  // 2^27, so the 2^32-scaled reciprocal, rounded up, is exact
+  auto block_of = [&](int page) { return static_cast<int>((static_cast<uint64_t>(page) * spb_inv) >> 32); };
+  auto entry = [&](int b, int idx) {
+    return idx < p.max_blocks_per_seq ? __ldg(p.block_table + b * p.bt_stride + idx) : 0;
+  };
+  const int pg0 = (c.p + c.off) * kUP;
+  int npg = kUP;
+  if (c.p == c.P - 1) {  // only a sequence's last unit can be short
+    const int L = max(__ldg(p.seq_lens + c.b), 0);
+    npg = min(kUP, min((L + kPageTokens - 1) / kPageTokens, p.max_blocks_per_seq * spb) - pg0);
+  }
+  int skip = 0;
+  if constexpr (kMod) skip = mod_skip_pages(p, c.b, pg0, c.p == 0);
+  const int e0 = block_of(pg0);
+  if (c.b != f.bt_b || e0 < f.bt_e0) {  // (another kv head starts over)
+    f.bt_b = c.b;
+    f.bt_e0 = e0;
+    f.bt_reg = entry(c.b, e0 + lane);
+    f.bt_next = entry(c.b, e0 + 32 + lane);
+  } else if (e0 >= f.bt_e0 + 32) {
+    f.bt_e0 += 32;
+    f.bt_reg = f.bt_next;
+    f.bt_next = entry(c.b, f.bt_e0 + 32 + lane);
+  }
+  // lane u < kUP: byte offset of page u's tile in either cache half
+  const int pg = pg0 + min(lane, npg - 1), e = block_of(pg);
+  // (shuffles take the lane index modulo 32)
+  const int b_lo = __shfl_sync(0xffffffffu, f.bt_reg, e - f.bt_e0);
+  const int b_hi = __shfl_sync(0xffffffffu, f.bt_next, e - f.bt_e0);
+  int blk = e - f.bt_e0 < 32 ? b_lo : b_hi;
+  if (blk < 0 || blk >= p.num_blocks) {
+    if (lane >= skip && lane < npg) set_status(p.status, PS_DEV_BLOCK_OUT_OF_RANGE);
+    blk = 0;
+  }
+  const int64_t tile = blk * p.c_sblock + c.h * p.c_shead + (pg - e * spb) * kFp4TileBytes;
+  const char* kbase = static_cast<const char*>(p.key_cache);
+  const char* vbase = static_cast<const char*>(p.value_cache);
+  const uint32_t dst = smem_u32(wsm + stage * SB) + lane * 16;
+#pragma unroll
+  for (int u = 0; u < kUP; ++u) {
+    const int64_t off = __shfl_sync(0xffffffffu, tile, u) + lane * 16;
+    if (u >= skip && u < npg) {
+      cp_async16(dst + u * kFp4TileBytes, kbase + off, kv_policy);
+      cp_async16(dst + u * kFp4TileBytes + 512, kbase + off + 512, kv_policy);
+      cp_async16(dst + (kUP + u) * kFp4TileBytes, vbase + off, kv_policy);
+      cp_async16(dst + (kUP + u) * kFp4TileBytes + 512, vbase + off + 512, kv_policy);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * kUP; i += 4) {  // tile i + lane / 8 of K tiles, then V tiles
+    const int x = i + (lane >> 3), u = x < kUP ? x : x - kUP;
+    const int64_t off = __shfl_sync(0xffffffffu, tile, u) + kFp4CodeBytes + (lane & 7) * 16;
+    if (u >= skip && u < npg)
+      cp_async16(smem_u32(wsm + stage * SB) + x * kFp4TileBytes + kFp4CodeBytes + (lane & 7) * 16,
+                 (x < kUP ? kbase : vbase) + off, kv_policy);
+  }
+  if (f.k == 0 || c.p == 0) {  // a segment starts for this warp: its query rows
+    const int qrow = p.qsl ? __ldg(p.qsl + c.b) : c.b;
+    const uint16_t* q =
+        reinterpret_cast<const uint16_t*>(p.q) + qrow * p.q_st + static_cast<int64_t>(c.h) * p.group * p.q_sh;
+    const uint32_t qdst = smem_u32(wq + (f.pseg % D) * fp4_qslot_bytes<NT>());
+    for (int i = lane; i < p.group * 16; i += 32)
+      cp_async16(qdst + i * 16, q + (i >> 4) * p.q_sh + (i & 15) * 8);
+    ++f.pseg;
+  }
+  cp_async_arrive(full + stage);
+  ++f.k;
+  fp4_next<kMod, kUP * kPageTokens>(f.pc, p, prefix, f.end);
+}
+
+// A copying warp: keeps the rings of kFp4Feeds streaming warps full.
+template <int NT, bool kMod>
+__device__ __forceinline__ void fp4_copy_warp(const DecodeParams& p, const Tables& tb, int64_t total, int64_t gw0,
+                                              uint8_t* smem, uint8_t* qslots, uint64_t* full, uint64_t* empty,
+                                              int first, int lane) {
+  constexpr int D = kFp4Stages;
+  constexpr int kUnitTokens = fp4_pages<NT>() * kPageTokens;
+  const int spb = p.block_size / kPageTokens;
+  const uint64_t spb_inv = ((1ull << 32) + spb - 1) / spb;
+  const uint64_t kv_policy = l2_policy_evict_first();
+  Fp4Feed f[kFp4Feeds];
+#pragma unroll
+  for (int i = 0; i < kFp4Feeds; ++i) {
+    const int64_t start = min(total, (gw0 + i) * tb.Qc);
+    f[i].end = min(total, start + tb.Qc);
+    f[i].k = f[i].pseg = f[i].bt_e0 = f[i].bt_reg = f[i].bt_next = 0;
+    f[i].bt_b = -1;
+    f[i].pc.v = f[i].end;
+    if (start < f[i].end) f[i].pc = fp4_seek<kMod, kUnitTokens>(start, f[i].end, p, tb.prefix);
+  }
+  long long since = clock64();
+  while (true) {
+    bool more = false, copied = false;
+#pragma unroll
+    for (int i = 0; i < kFp4Feeds; ++i) {
+      if (f[i].pc.v >= f[i].end) continue;
+      more = true;
+      const int ring = (first + i) * D;
+      const int use = f[i].k / D;  // earlier uses of the stage, the last of which must have been released
+      int free = 1;
+      if (use > 0) {
+        if (lane == 0) free = mbar_test(empty + ring + f[i].k % D, static_cast<uint32_t>((use - 1) & 1));
+        free = __shfl_sync(0xffffffffu, free, 0);
+        __syncwarp();  // lane 0's acquire orders the whole warp's copies
+      }
+      if (!free) continue;
+      fp4_copy_unit<NT, kMod>(f[i], p, smem + ring * fp4_stage_bytes<NT>(), qslots + ring * fp4_qslot_bytes<NT>(),
+                              full + ring, tb.prefix, spb_inv, kv_policy, lane);
+      copied = true;
+    }
+    if (!more) break;
+    if (copied) {
+      since = clock64();
+    } else if (clock64() - since > kWaitLimitCycles) {
+      if (lane == 0) set_status(p.status, PS_DEV_WAIT_TIMEOUT);
+      break;
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// A streaming warp attends over the units of list positions [start, end).
 template <bool kBF16, int NT, bool kMod>
 __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Tables& tb, int64_t start, int64_t end,
-                                                 int64_t gw, uint8_t* wsm, uint8_t* wq, int lane) {
+                                                 int64_t gw, uint8_t* wsm, uint8_t* wq, uint64_t* full,
+                                                 uint64_t* empty, int lane) {
   constexpr int kRec = 8 * NT;
   constexpr int D = kFp4Stages;
   constexpr int kUP = fp4_pages<NT>();
   constexpr int kUnitTokens = kUP * kPageTokens;
   constexpr int SB = fp4_stage_bytes<NT>();
-  static_assert(kUP % 2 == 0 && kUP <= 32, "the scale rows of a unit are copied four tiles at a time");
-  static_assert(SB % 128 == 0, "stage alignment");
   const int Hkv = p.num_kv_heads;
-  const int spb = p.block_size / kPageTokens;
   const int group = p.group;
   const float k_scale = p.k_scale ? __ldg(p.k_scale) : 1.f;
   const float v_scale = p.v_scale ? __ldg(p.v_scale) : 1.f;
   const float scale_log2 = p.scale_log2 * k_scale;
-
-  // Block-table entries are held 64 at a time, [bt_e0, bt_e0 + 64) of sequence
-  // bt_b: the second half is loaded when the first comes into use, so that
-  // only a new sequence waits for its entries.
-  int bt_b = -1, bt_e0 = 0, bt_reg = 0, bt_next = 0;
-  int pseg = 0;
-  // page / spb without a division: spb = block_size / 16 is in [1, 16] and a
-  // page index below 2^27, so the 2^32-scaled reciprocal, rounded up, is exact
-  const uint64_t spb_inv = ((1ull << 32) + spb - 1) / spb;
-  auto block_of = [&](int page) { return static_cast<int>((static_cast<uint64_t>(page) * spb_inv) >> 32); };
-  auto entry = [&](int b, int idx) {
-    return idx < p.max_blocks_per_seq ? __ldg(p.block_table + b * p.bt_stride + idx) : 0;
-  };
-  const uint64_t kv_policy = l2_policy_evict_first();
-  // Issue the tiles of unit c into `stage` as one group of asynchronous copies:
-  // two 512-byte warp copies of codes per tile, and one warp copy for the
-  // scale rows (128 bytes) of four tiles.  Pages past the sequence or below the
-  // visible range are neither copied nor looked up (their tokens are masked).
-  // (Bulk copies, one per tile, cost a warp 140 cycles each to issue -- their
-  // operands are uniform, so lanes take turns -- 1,130 a unit of four pages, a
-  // quarter of its time.)
-  auto issue = [&](int stage, const Fp4Cursor& c, bool seg_start) {
-    const int pg0 = (c.p + c.off) * kUP;
-    int npg = kUP;
-    if (c.p == c.P - 1) {  // only a sequence's last unit can be short
-      const int L = max(__ldg(p.seq_lens + c.b), 0);
-      npg = min(kUP, min((L + kPageTokens - 1) / kPageTokens, p.max_blocks_per_seq * spb) - pg0);
-    }
-    int skip = 0;
-    if constexpr (kMod) skip = mod_skip_pages(p, c.b, pg0, c.p == 0);
-    const int e0 = block_of(pg0);
-    if (c.b != bt_b || e0 < bt_e0) {  // (another kv head starts over)
-      bt_b = c.b;
-      bt_e0 = e0;
-      bt_reg = entry(c.b, e0 + lane);
-      bt_next = entry(c.b, e0 + 32 + lane);
-    } else if (e0 >= bt_e0 + 32) {
-      bt_e0 += 32;
-      bt_reg = bt_next;
-      bt_next = entry(c.b, bt_e0 + 32 + lane);
-    }
-    // lane u < kUP: byte offset of page u's tile in either cache half
-    const int pg = pg0 + min(lane, npg - 1), e = block_of(pg);
-    // (shuffles take the lane index modulo 32)
-    const int b_lo = __shfl_sync(0xffffffffu, bt_reg, e - bt_e0), b_hi = __shfl_sync(0xffffffffu, bt_next, e - bt_e0);
-    int blk = e - bt_e0 < 32 ? b_lo : b_hi;
-    if (blk < 0 || blk >= p.num_blocks) {
-      if (lane >= skip && lane < npg) set_status(p.status, PS_DEV_BLOCK_OUT_OF_RANGE);
-      blk = 0;
-    }
-    const int64_t tile = blk * p.c_sblock + c.h * p.c_shead + (pg - e * spb) * kFp4TileBytes;
-    const char* kbase = static_cast<const char*>(p.key_cache);
-    const char* vbase = static_cast<const char*>(p.value_cache);
-    const uint32_t dst = smem_u32(wsm + stage * SB) + lane * 16;
-#pragma unroll
-    for (int u = 0; u < kUP; ++u) {
-      const int64_t off = __shfl_sync(0xffffffffu, tile, u) + lane * 16;
-      if (u >= skip && u < npg) {
-        cp_async16(dst + u * kFp4TileBytes, kbase + off, kv_policy);
-        cp_async16(dst + u * kFp4TileBytes + 512, kbase + off + 512, kv_policy);
-        cp_async16(dst + (kUP + u) * kFp4TileBytes, vbase + off, kv_policy);
-        cp_async16(dst + (kUP + u) * kFp4TileBytes + 512, vbase + off + 512, kv_policy);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * kUP; i += 4) {  // tile i + lane / 8 of K tiles, then V tiles
-      const int x = i + (lane >> 3), u = x < kUP ? x : x - kUP;
-      const int64_t off = __shfl_sync(0xffffffffu, tile, u) + kFp4CodeBytes + (lane & 7) * 16;
-      if (u >= skip && u < npg)
-        cp_async16(smem_u32(wsm + stage * SB) + x * kFp4TileBytes + kFp4CodeBytes + (lane & 7) * 16,
-                   (x < kUP ? kbase : vbase) + off, kv_policy);
-    }
-    if (seg_start) {
-      const int qrow = p.qsl ? __ldg(p.qsl + c.b) : c.b;
-      const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + qrow * p.q_st + static_cast<int64_t>(c.h) * group * p.q_sh;
-      const uint32_t qdst = smem_u32(wq + (pseg % D) * fp4_qslot_bytes<NT>());
-      for (int i = lane; i < group * 16; i += 32)
-        cp_async16(qdst + i * 16, q + (i >> 4) * p.q_sh + (i & 15) * 8);
-      ++pseg;
-    }
-    cp_async_commit();
-  };
-
-  Fp4Cursor pc = fp4_seek<kMod, kUnitTokens>(start, end, p, tb.prefix);
-  if (pc.v >= end) return;  // empty positions only
-  Fp4Cursor cc = pc;
-  // pc is the next unit to copy, cc the next to attend over
-#pragma unroll 1
-  for (int k = 0; k < D; ++k) {
-    if (pc.v < end) {
-      issue(k, pc, k == 0 || pc.p == 0);
-      fp4_next<kMod, kUnitTokens>(pc, p, tb.prefix, end);
-    } else {
-      cp_async_commit();
-    }
-  }
+  Fp4Cursor cc = fp4_seek<kMod, kUnitTokens>(start, end, p, tb.prefix);  // next unit to attend over
 
   const int g = lane >> 2, t = lane & 3;
   uint32_t qf[NT][8][2];
@@ -283,10 +360,10 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
   for (int k = 0; cc.v < end; ++k) {
     const int stage = k % D;
     uint8_t* st = wsm + stage * SB;
-    // one group is committed per iteration, so the oldest D - 1 or fewer are
-    // outstanding exactly when this unit's has arrived
-    cp_async_wait<D - 1>();
-    __syncwarp();
+    if (!mbar_wait_bounded(full + stage, static_cast<uint32_t>((k / D) & 1))) {
+      if (lane == 0) set_status(p.status, PS_DEV_WAIT_TIMEOUT);
+      return;
+    }
 
     // ---- segment start: query fragments, reset state ---------------------------
     if (k == 0 || cc.p == 0) {
@@ -537,13 +614,8 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
     }
     __syncwarp();
 
-    // ---- refill this stage with the unit D ahead -----------------------------------
-    if (pc.v < end) {
-      issue(stage, pc, pc.p == 0);
-      fp4_next<kMod, kUnitTokens>(pc, p, tb.prefix, end);
-    } else {
-      cp_async_commit();
-    }
+    // ---- the stage may be filled again ----------------------------------------
+    if (lane == 0) mbar_arrive(empty + stage);
 
     // ---- segment end: finalize ---------------------------------------------------
     const Fp4Cursor at = cc;
@@ -593,21 +665,28 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
   for (int i = 1; i <= 2; ++i)
     if (pending & i) {
       const Fp4Cursor c = fp4_locate<kMod, kUnitTokens>(i == 1 ? start : end - 1, p, tb.prefix);
-      merge_split<kBF16, kRec>(p, fp4_split(c, Hkv, tb.Qc), gw, lane);
+      merge_split<kBF16, kRec, false>(p, fp4_split(c, Hkv, tb.Qc), gw, lane);
     }
 }
 
 template <bool kBF16, int NT, bool kMod>
-__global__ void __launch_bounds__(fp4_warps<NT>() * 32, 1) paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(fp4_threads<NT>(), 1) paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int D = kFp4Stages, W = fp4_warps<NT>();
   constexpr int kUP = fp4_pages<NT>(), kUnitTokens = kUP * kPageTokens, SB = fp4_stage_bytes<NT>();
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* qslots = smem + W * D * SB;
-  int* prefix = reinterpret_cast<int*>(qslots + W * D * fp4_qslot_bytes<NT>());
-  __shared__ int s_warp_tot[W];
+  uint64_t* full = reinterpret_cast<uint64_t*>(qslots + W * D * fp4_qslot_bytes<NT>());
+  uint64_t* empty = full + W * D;
+  int* prefix = reinterpret_cast<int*>(empty + W * D);
+  __shared__ int s_warp_tot[fp4_threads<NT>() / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int B = p.num_seqs, Hkv = p.num_kv_heads;
   const int spb = p.block_size / kPageTokens;
+  if (tid < W * D) {
+    mbar_init(full + tid, 32);  // every lane of the copying warp
+    mbar_init(empty + tid, 1);
+    fence_mbar_init();
+  }
   // the launch overlaps the previous kernel in the stream up to here
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
@@ -660,11 +739,22 @@ __global__ void __launch_bounds__(fp4_warps<NT>() * 32, 1) paged_decode_fp4_kern
     if (p.lse) p.lse[qh * p.lse_sh + qrow * p.lse_st] = -INFINITY;
   }
 
-  const int64_t gw = static_cast<int64_t>(blockIdx.x) * W + warp;
-  const int64_t start = min(total, gw * tb.Qc), end = min(total, start + tb.Qc);
-  if (start < end)
-    stream_range_fp4<kBF16, NT, kMod>(p, tb, start, end, gw, smem + warp * D * SB,
-                                      qslots + warp * D * fp4_qslot_bytes<NT>(), lane);
+  // (the scan's barriers order the mbarriers' initialisation)
+  if (warp >= W) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp4CopyRegs));
+    const int first = (warp - W) * kFp4Feeds;
+    if (first < W)
+      fp4_copy_warp<NT, kMod>(p, tb, total, static_cast<int64_t>(blockIdx.x) * W + first, smem, qslots, full, empty,
+                              first, lane);
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp4StreamRegs));
+    const int64_t gw = static_cast<int64_t>(blockIdx.x) * W + warp;
+    const int64_t start = min(total, gw * tb.Qc), end = min(total, start + tb.Qc);
+    if (start < end)
+      stream_range_fp4<kBF16, NT, kMod>(p, tb, start, end, gw, smem + warp * D * SB,
+                                        qslots + warp * D * fp4_qslot_bytes<NT>(), full + warp * D, empty + warp * D,
+                                        lane);
+  }
 }
 
 template <bool kBF16, int NT, bool kMod>
@@ -683,7 +773,7 @@ static int launch_fp4(const DecodeParams& p, int sm_count, cudaStream_t stream) 
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sm_count);
-  cfg.blockDim = dim3(fp4_warps<NT>() * 32);
+  cfg.blockDim = dim3(fp4_threads<NT>());
   cfg.dynamicSmemBytes = base + static_cast<size_t>(p.num_seqs + 1) * 4;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -519,7 +519,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 // a one-sequence call.  The loops stay rolled: code that runs once per segment is
 // fetched from L2.  More than 32 sources are folded in with a running maximum.
 template <bool kBF16, int kRec, bool kToRecord, int NR>
-__device__ __noinline__ void combine_split_rows(const DecodeParams& p, int64_t slot0, int n, int stride, int j0,
+__device__ __forceinline__ void combine_split_rows(const DecodeParams& p, int64_t slot0, int n, int stride, int j0,
                                                 int nrows, int b, int h, int lane) {
   constexpr int S = 16 / NR;
   constexpr float kLog2e = 1.4426950408889634f;
@@ -614,14 +614,28 @@ __device__ __noinline__ void combine_split_rows(const DecodeParams& p, int64_t s
   }
 }
 template <bool kBF16, int kRec, bool kToRecord>
-__device__ __forceinline__ void combine_split(const DecodeParams& p, int64_t slot0, int n, int stride, int nrows,
-                                              int b, int h, int lane) {
+__device__ __forceinline__ void combine_split_inline(const DecodeParams& p, int64_t slot0, int n, int stride, int nrows,
+                                                     int b, int h, int lane) {
   if (nrows <= 2) {
     combine_split_rows<kBF16, kRec, kToRecord, 2>(p, slot0, n, stride, 0, nrows, b, h, lane);
   } else {
     for (int j0 = 0; j0 < nrows; j0 += 8)
       combine_split_rows<kBF16, kRec, kToRecord, 8>(p, slot0, n, stride, j0, min(8, nrows - j0), b, h, lane);
   }
+}
+// kCall: as a function (a kernel whose warps split the registers unevenly has none)
+template <bool kBF16, int kRec, bool kToRecord>
+__device__ __noinline__ void combine_split_call(const DecodeParams& p, int64_t slot0, int n, int stride, int nrows, int b,
+                                                int h, int lane) {
+  combine_split_inline<kBF16, kRec, kToRecord>(p, slot0, n, stride, nrows, b, h, lane);
+}
+template <bool kBF16, int kRec, bool kToRecord, bool kCall>
+__device__ __forceinline__ void combine_split(const DecodeParams& p, int64_t slot0, int n, int stride, int nrows,
+                                              int b, int h, int lane) {
+  if constexpr (kCall)
+    combine_split_call<kBF16, kRec, kToRecord>(p, slot0, n, stride, nrows, b, h, lane);
+  else
+    combine_split_inline<kBF16, kRec, kToRecord>(p, slot0, n, stride, nrows, b, h, lane);
 }
 
 // Count one contribution into *counter; true (for the whole warp) for the last
@@ -670,7 +684,7 @@ __device__ __forceinline__ bool count_record(const DecodeParams& p, const SplitS
   return count_split(chunk_counter(p, g, chunk), min(size, g.nsplit - chunk * size), lane);
 }
 
-template <bool kBF16, int kRec>
+template <bool kBF16, int kRec, bool kCall = true>
 __device__ __forceinline__ void merge_split(const DecodeParams& p, const SplitSeg& g, int64_t gw, int lane) {
   const int64_t slot0 = g.first_w + g.unit;
   int32_t* counter = p.counters + g.unit;
@@ -680,10 +694,10 @@ __device__ __forceinline__ void merge_split(const DecodeParams& p, const SplitSe
     const int chunk = static_cast<int>(gw - g.first_w) / size, members = min(size, g.nsplit - chunk * size);
     if (lane == 0) *chunk_counter(p, g, chunk) = 0;
     if (members > 1)
-      combine_split<kBF16, kRec, true>(p, slot0 + chunk * size, members, 1, p.group, g.b, g.h, lane);
+      combine_split<kBF16, kRec, true, kCall>(p, slot0 + chunk * size, members, 1, p.group, g.b, g.h, lane);
     if (!count_split(counter, chunks, lane)) return;
   }
-  combine_split<kBF16, kRec, false>(p, slot0, chunks > 1 ? chunks : g.nsplit, chunks > 1 ? size : 1, p.group, g.b,
+  combine_split<kBF16, kRec, false, kCall>(p, slot0, chunks > 1 ? chunks : g.nsplit, chunks > 1 ? size : 1, p.group, g.b,
                                     g.h, lane);
   if (lane == 0) *counter = 0;
 }
