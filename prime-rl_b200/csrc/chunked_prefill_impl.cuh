@@ -175,7 +175,7 @@ struct UnitInfo {
 // Score modifiers: the first visible key of query row `tok` at position `pos`.
 __device__ __forceinline__ int mod_row_low(const PrefillParams& p, int qrow, int pos) {
   int lo = 0;
-  if (p.mod.window_left >= 0) lo = max(lo, pos - p.mod.window_left);
+  if (p.mod.window_left >= 0) lo = max(lo, max(pos, 0) - p.mod.window_left);  // (no overflow: a bad length's pos)
   if (p.mod.key_start != nullptr) lo = max(lo, __ldg(p.mod.key_start + qrow));
   return lo;
 }

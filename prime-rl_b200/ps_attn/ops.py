@@ -620,8 +620,9 @@ def dequant_gather(key_cache: torch.Tensor, value_cache: torch.Tensor, block_tab
         raise ValueError("dequant_gather reads an fp8 or nvfp4 cache")
     B = seq_lens.shape[0]
     nb, bs, hkv, d = key_cache.shape
-    if is_nvfp4_cache(key_cache):
-        nb, hkv, bs, d = key_cache.shape[0], key_cache.shape[1], key_cache.shape[2], 128
+    fp4 = is_nvfp4_cache(key_cache)
+    if fp4:
+        hkv, bs, d = bs, hkv, 128
     dev = key_cache.device
     if out is None:
         kd = torch.empty(B * max_pages, bs, hkv, d, dtype=dtype, device=dev)
@@ -638,9 +639,27 @@ def dequant_gather(key_cache: torch.Tensor, value_cache: torch.Tensor, block_tab
         bt = out[2] if len(out) > 2 else None
     if B == 0 or max_pages == 0:
         return kd, vd, bt
-    q_like = kd.flatten(0, 1)  # (not read)
-    pr = _problem(q_like, key_cache, value_cache, block_table, seq_lens, None, 1.0, q_like, None,
-                  status=status, k_scale=k_scale, v_scale=v_scale)
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"scratch dtype {dtype} unsupported (fp16/bf16)")
+    if key_cache.stride() != value_cache.stride() or key_cache.shape != value_cache.shape:
+        raise ValueError("key_cache and value_cache must have the same shape and strides")
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise ValueError("block_table and seq_lens must be int32")
+    if block_table.stride(-1) != 1 or not seq_lens.is_contiguous() or key_cache.stride(-1) != 1:
+        raise ValueError("block_table rows, seq_lens and the caches' last dimension must be contiguous")
+    if status is not None and (status.dtype != torch.int32 or not status.is_cuda):
+        raise ValueError("status must be a CUDA int32 tensor")
+    if fp4:
+        _check_nvfp4(key_cache, value_cache)
+        s_block, s_head, s_slot = key_cache.stride()[:3]
+    else:
+        s_block, s_slot, s_head = key_cache.stride()[:3]
+    pr = _lib.PagedProblem.from_buffer_copy(_lib.PAGED_PROBLEM_STRUCT.pack(
+        0, 0, 0, key_cache.data_ptr(), value_cache.data_ptr(), s_block, s_slot, s_head, nb,
+        block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), 0, B,
+        0, 0, 0, 0, 0, 0, hkv, hkv, d, bs, _DTYPES[dtype], 1.0, 0,
+        status.data_ptr() if status is not None else 0, 0, 0, 0, 0, 0, 0, 0,
+        _lib.PS_KV_NVFP4 if fp4 else _lib.PS_KV_FP8_E4M3, _scale_ptr(k_scale) or 0, _scale_ptr(v_scale) or 0))
     _launch(dev, lib.ps_kv_dequant_gather, ctypes.byref(pr), max_pages, kd.data_ptr(), vd.data_ptr(),
             _stream_ptr(dev))
     return kd, vd, bt
