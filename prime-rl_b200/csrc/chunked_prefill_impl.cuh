@@ -137,9 +137,17 @@ struct PrefillSmem {
   static constexpr int xchg_off = misc_off + 32;  // (after them: tiles[2] of the units, score modifiers)
   // score modifiers: (first, last) visible key of each thread's two rows, int2 [256][2]
   static constexpr int range_off = xchg_off + 2 * (2 * 2 * 128 * 4);
-  static constexpr int table_off = range_off + 256 * 2 * 8;
+  // sequences in the order their units are listed (kOrderSeqs or fewer), and their lengths
+  static constexpr int order_off = range_off + 256 * 2 * 8;
+  static constexpr int table_off = order_off + 2 * 128 * 4;
   static constexpr int bytes_before_table = table_off;
 };
+
+// Batches of at most this many sequences list them by falling length when there
+// are more units than CTAs, so that no CTA starts a long one last (24 follow-up
+// turns of 77 tokens over 129-1,999 cached ones, 192 units: 81 us in batch order,
+// 73 so).  Larger batches have units enough to even out.
+constexpr int kOrderSeqs = 128;
 
 struct PBars {
   uint64_t* q_full;
@@ -200,7 +208,7 @@ __device__ __forceinline__ void mod_unit_range(const PrefillParams& p, UnitInfo&
 
 // Units are (sequence, M-tile pair, kv head); within a sequence the pairs are
 // enumerated from the last (longest causal range) to the first.
-__device__ __forceinline__ UnitInfo unit_info(const PrefillParams& p, const int* prefix, int u) {
+__device__ __forceinline__ UnitInfo unit_info(const PrefillParams& p, const int* prefix, const int* order, int u) {
   UnitInfo ui;
   const int pu = u / p.num_kv_heads;
   ui.h = u - pu * p.num_kv_heads;
@@ -209,9 +217,10 @@ __device__ __forceinline__ UnitInfo unit_info(const PrefillParams& p, const int*
     const int mid = (lo + hi + 1) >> 1;
     if (prefix[mid] <= pu) lo = mid; else hi = mid - 1;
   }
-  ui.b = lo;
   const int npairs = prefix[lo + 1] - prefix[lo];
   const int mp = npairs - 1 - (pu - prefix[lo]);
+  if (order != nullptr) lo = order[lo];
+  ui.b = lo;
   ui.qrow0 = __ldg(p.qsl + lo);
   ui.qlen = __ldg(p.qsl + lo + 1) - ui.qrow0;
   const int L = __ldg(p.seq_lens + lo);
@@ -399,6 +408,35 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   const int total_units = prefix[B] * p.num_kv_heads;
+  int* order = nullptr;
+  if (B > 1 && B <= kOrderSeqs && total_units > static_cast<int>(gridDim.x)) {
+    // rank of each sequence by falling length (ties in batch order), then the
+    // pairs' prefix in that order
+    order = reinterpret_cast<int*>(smem + L::order_off);
+    int* lens = order + kOrderSeqs;
+    const int len = tid < B ? __ldg(p.seq_lens + tid) : 0;
+    if (tid < B) lens[tid] = len;
+    __syncthreads();
+    int rank = 0;
+    for (int b = 0; b < B; ++b) rank += (lens[b] > len || (lens[b] == len && b < tid)) ? 1 : 0;
+    if (tid < B) order[rank] = tid;
+    __syncthreads();
+    if (warp == 0) {
+      int run = 0;
+      for (int r0 = 0; r0 < B; r0 += 32) {
+        const int n = r0 + lane < B ? pairs_of(order[r0 + lane]) : 0;
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += v;
+        }
+        if (r0 + lane < B) prefix[r0 + lane] = run + sum - n;
+        run += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    __syncthreads();
+  }
 
   uint8_t* sQ = smem + L::q_off;
   uint8_t* sK = smem + L::k_off;
@@ -412,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int t = 0, uit = 0;
     int bt_b = -1, bt_e0 = 0, bt_reg = 0;
     for (int u = blockIdx.x; u < total_units && !*abort_flag; ++uit) {
-      UnitInfo ui = unit_info(p, prefix, u);
+      UnitInfo ui = unit_info(p, prefix, order, u);
       if constexpr (kMod) mod_unit_range(p, ui, lane);
       if (!pwait(bars.q_empty, (uit & 1) ^ 1, abort_flag, p.status)) break;
       if (lane == 0) {
@@ -512,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int t = 0, uit = 0;
       bool ok = true;
       for (int u = blockIdx.x; u < total_units && ok; ++uit) {
-        UnitInfo ui = unit_info(p, prefix, u);
+        UnitInfo ui = unit_info(p, prefix, order, u);
         if (!pwait(bars.q_full, static_cast<uint32_t>(uit & 1), abort_flag, p.status)) break;
         if constexpr (kMod) ui.ntiles = s_ntiles[uit & 1];
         tc::fence_after_sync();
@@ -572,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float cap_u = cap_in * 0.34657359f;
     const float cap_fast = cap_u <= 1e4f ? 0.5f / cap_u : 0.f;
     for (int u = blockIdx.x; u < total_units; ++uit) {
-      UnitInfo ui = unit_info(p, prefix, u);
+      UnitInfo ui = unit_info(p, prefix, order, u);
       if constexpr (kMod) mod_unit_range(p, ui, lane);
       int tok[2], limit[2];
       // score modifiers: the rows' ranges are kept in shared memory (each thread
