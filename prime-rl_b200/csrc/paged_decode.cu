@@ -9,7 +9,7 @@ int64_t ps_decode_partial_slots(int num_seqs, int num_kv_heads, int sm_count, in
   // cascade mode, at most one prefix segment per (sequence, kv head) more
   const int64_t units = static_cast<int64_t>(num_seqs) * num_kv_heads * (cascade ? 2 : 1);
   return static_cast<int64_t>(sm_count) * ps::kDecodeCtasPerSm *
-             (fp4 ? ps::kDecodeFp4MaxWarps : fp8 ? ps::kDecodeFp8Warps : ps::kDecodeWarps) + units;
+             (fp4 ? ps::kDecodeFp4Warps : fp8 ? ps::kDecodeFp8Warps : ps::kDecodeWarps) + units;
 }
 
 namespace ps {

@@ -5,8 +5,8 @@
 // A page-head is 2304 bytes (K tile + V tile) against 8192 in 16 bits, so
 // what bounds the kernel is the instruction stream that turns codes into
 // tensor-core operands, not HBM.  Hence:
-//   - the unit of work is a few pages of one (sequence, kv head): one
-//     wait, one maximum and one rescale per unit;
+//   - the unit of work is four pages of one (sequence, kv head): one wait, one
+//     maximum and one rescale per unit; four more warps of a CTA do the copying;
 //   - the tile layout (nvfp4.cuh) is the fragment order: a lane's K codes are
 //     two 16-byte loads and its V codes two more, without ldmatrix;
 //   - K: the reduction dims of the 8 MMA steps are permuted so that a lane
@@ -20,43 +20,34 @@
 //     P is exact.  The query is scaled by a power of two per head into [-2, 2]
 //     so that no 16-bit query overflows f16; the power goes into the score
 //     scale.  P is rounded to f16 (2^-11).
+// 40 sequences of 2k-32k tokens, 64 / 8 heads (459 MB): 112 us, 4.1 TB/s, 63 % of the
+// measured copy rate; without the conversions, the scaling and the nibble
+// interleaving 23 % less, without the MMAs 1 %.  64 of 1k-4k, 16 / 8 heads (158 MB):
+// 48 us; one of 1,531: 13 us.
 #include "nvfp4.cuh"
 #include "paged_decode_impl.cuh"
 
 namespace ps {
 
-#ifndef PS_DECODE_FP4_PAGES
-#define PS_DECODE_FP4_PAGES 4
-#endif
-#ifndef PS_DECODE_FP4_PAGES2
-#define PS_DECODE_FP4_PAGES2 4
-#endif
 constexpr int kFp4Stages = kDecodeFp4Stages;
-// Pages of one unit and warps of a CTA, by query-column tiles.
-template <int NT>
-__host__ __device__ constexpr int fp4_pages() {
-  return NT == 1 ? PS_DECODE_FP4_PAGES : PS_DECODE_FP4_PAGES2;
-}
-template <int NT>
-__host__ __device__ constexpr int fp4_warps() {
-  return NT == 1 ? kDecodeFp4Warps : kDecodeFp4Warps2;
-}
+constexpr int kFp4Warps = kDecodeFp4Warps;   // streaming warps
+// Pages of one unit: a unit costs a warp 180 instructions besides 260 a page, and
+// four pages are what two stages of eight warps leave room for (units of two
+// pages: 161 us where four take 134, before the copying warps).
+constexpr int kFp4UnitPages = 4;
+constexpr int kFp4UnitTokens = kFp4UnitPages * kPageTokens;
+constexpr int kFp4StageBytes = 2 * kFp4UnitPages * kFp4TileBytes;  // K tiles, then V tiles
+static_assert(kFp4UnitPages % 2 == 0, "the scale rows of a unit are copied four tiles at a time");
+static_assert(kFp4StageBytes % 128 == 0, "stage alignment");
 // Four more warps copy for the streaming warps, two each.  Copying is addresses and
 // shuffles with little to overlap them, 1,000 of the 4,400 cycles a unit took a
 // warp that did both.  Registers: 384 threads start with 168 each; the
 // streaming warps take the copying warps' share (256 * 216 + 128 * 72 = 384 * 168).
-constexpr int kFp4Feeds = 2;
+constexpr int kFp4CopyWarps = 4, kFp4Feeds = kFp4Warps / kFp4CopyWarps;
+constexpr int kFp4Threads = (kFp4Warps + kFp4CopyWarps) * 32;
 constexpr int kFp4StreamRegs = 216, kFp4CopyRegs = 72;
-template <int NT>
-__host__ __device__ constexpr int fp4_threads() {
-  static_assert(fp4_warps<NT>() == 8, "two warpgroups of streaming warps, one of copying warps");
-  static_assert(256 * kFp4StreamRegs + 128 * kFp4CopyRegs <= 384 * 168, "the launch's registers");
-  return (fp4_warps<NT>() + 4) * 32;
-}
-template <int NT>
-__host__ __device__ constexpr int fp4_stage_bytes() {  // K tiles, then V tiles
-  return 2 * fp4_pages<NT>() * kFp4TileBytes;
-}
+static_assert(kFp4Warps == 8, "two warpgroups of streaming warps, one of copying warps");
+static_assert(256 * kFp4StreamRegs + 128 * kFp4CopyRegs <= 384 * 168, "the launch's registers");
 
 // 16 bytes global -> shared, asynchronous, through L2 only.
 __device__ __forceinline__ void cp_async16(uint32_t smem_dst, const void* gsrc, uint64_t policy) {
@@ -94,7 +85,7 @@ __host__ __device__ constexpr int fp4_qslot_bytes() {
 template <int NT>
 __host__ __device__ constexpr int fp4_smem_bytes_before_table() {
   // stages | per-warp query slots | full and empty barriers
-  return fp4_warps<NT>() * kFp4Stages * (fp4_stage_bytes<NT>() + fp4_qslot_bytes<NT>() + 16);
+  return kFp4Warps * kFp4Stages * (kFp4StageBytes + fp4_qslot_bytes<NT>() + 16);
 }
 
 // Position in the list.  A segment (sequence, kv head) of P units takes P +
@@ -199,10 +190,8 @@ __device__ __forceinline__ void fp4_copy_unit(Fp4Feed& f, const DecodeParams& p,
                                               uint64_t* full, const int* prefix, uint64_t spb_inv, uint64_t kv_policy,
                                               int lane) {
   constexpr int D = kFp4Stages;
-  constexpr int kUP = fp4_pages<NT>();
-  constexpr int SB = fp4_stage_bytes<NT>();
-  static_assert(kUP % 2 == 0 && kUP <= 32, "the scale rows of a unit are copied four tiles at a time");
-  static_assert(SB % 128 == 0, "stage alignment");
+  constexpr int kUP = kFp4UnitPages;
+  constexpr int SB = kFp4StageBytes;
   const Fp4Cursor& c = f.pc;
   const int spb = p.block_size / kPageTokens;
   const int stage = f.k % D;
@@ -283,7 +272,7 @@ __device__ __forceinline__ void fp4_copy_warp(const DecodeParams& p, const Table
                                               uint8_t* smem, uint8_t* qslots, uint64_t* full, uint64_t* empty,
                                               int first, int lane) {
   constexpr int D = kFp4Stages;
-  constexpr int kUnitTokens = fp4_pages<NT>() * kPageTokens;
+  constexpr int kUnitTokens = kFp4UnitPages * kPageTokens;
   const int spb = p.block_size / kPageTokens;
   const uint64_t spb_inv = ((1ull << 32) + spb - 1) / spb;
   const uint64_t kv_policy = l2_policy_evict_first();
@@ -313,7 +302,7 @@ __device__ __forceinline__ void fp4_copy_warp(const DecodeParams& p, const Table
         __syncwarp();  // lane 0's acquire orders the whole warp's copies
       }
       if (!free) continue;
-      fp4_copy_unit<NT, kMod>(f[i], p, smem + ring * fp4_stage_bytes<NT>(), qslots + ring * fp4_qslot_bytes<NT>(),
+      fp4_copy_unit<NT, kMod>(f[i], p, smem + ring * kFp4StageBytes, qslots + ring * fp4_qslot_bytes<NT>(),
                               full + ring, tb.prefix, spb_inv, kv_policy, lane);
       copied = true;
     }
@@ -335,9 +324,9 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
                                                  uint64_t* empty, int lane) {
   constexpr int kRec = 8 * NT;
   constexpr int D = kFp4Stages;
-  constexpr int kUP = fp4_pages<NT>();
+  constexpr int kUP = kFp4UnitPages;
   constexpr int kUnitTokens = kUP * kPageTokens;
-  constexpr int SB = fp4_stage_bytes<NT>();
+  constexpr int SB = kFp4StageBytes;
   const int Hkv = p.num_kv_heads;
   const int group = p.group;
   const float k_scale = p.k_scale ? __ldg(p.k_scale) : 1.f;
@@ -670,15 +659,15 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
 }
 
 template <bool kBF16, int NT, bool kMod>
-__global__ void __launch_bounds__(fp4_threads<NT>(), 1) paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
-  constexpr int D = kFp4Stages, W = fp4_warps<NT>();
-  constexpr int kUP = fp4_pages<NT>(), kUnitTokens = kUP * kPageTokens, SB = fp4_stage_bytes<NT>();
+__global__ void __launch_bounds__(kFp4Threads, 1) paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
+  constexpr int D = kFp4Stages, W = kFp4Warps;
+  constexpr int kUP = kFp4UnitPages, kUnitTokens = kUP * kPageTokens, SB = kFp4StageBytes;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* qslots = smem + W * D * SB;
   uint64_t* full = reinterpret_cast<uint64_t*>(qslots + W * D * fp4_qslot_bytes<NT>());
   uint64_t* empty = full + W * D;
   int* prefix = reinterpret_cast<int*>(empty + W * D);
-  __shared__ int s_warp_tot[fp4_threads<NT>() / 32];
+  __shared__ int s_warp_tot[kFp4Threads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int B = p.num_seqs, Hkv = p.num_kv_heads;
   const int spb = p.block_size / kPageTokens;
@@ -773,7 +762,7 @@ static int launch_fp4(const DecodeParams& p, int sm_count, cudaStream_t stream) 
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sm_count);
-  cfg.blockDim = dim3(fp4_threads<NT>());
+  cfg.blockDim = dim3(kFp4Threads);
   cfg.dynamicSmemBytes = base + static_cast<size_t>(p.num_seqs + 1) * 4;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -117,19 +117,14 @@ constexpr int kDecodeWarps = PS_DECODE_WARPS;           // warps per CTA
 // so the same warps and stages as the 16-bit kernel
 constexpr int kDecodeFp8Warps = PS_DECODE_FP8_WARPS;
 constexpr int kDecodeFp8Stages = PS_DECODE_FP8_STAGES;
-// 4-bit (nvfp4) caches: a unit is four pages (9 KB)
+// 4-bit (nvfp4) caches: a unit is four pages (9 KB); four warps more do the copying
 #ifndef PS_DECODE_FP4_WARPS
 #define PS_DECODE_FP4_WARPS 8
 #endif
 #ifndef PS_DECODE_FP4_STAGES
 #define PS_DECODE_FP4_STAGES 2
 #endif
-#ifndef PS_DECODE_FP4_WARPS2
-#define PS_DECODE_FP4_WARPS2 8
-#endif
-constexpr int kDecodeFp4Warps = PS_DECODE_FP4_WARPS;    // GQA group <= 8
-constexpr int kDecodeFp4Warps2 = PS_DECODE_FP4_WARPS2;  // GQA group 9 to 16
-constexpr int kDecodeFp4MaxWarps = kDecodeFp4Warps > kDecodeFp4Warps2 ? kDecodeFp4Warps : kDecodeFp4Warps2;
+constexpr int kDecodeFp4Warps = PS_DECODE_FP4_WARPS;
 constexpr int kDecodeFp4Stages = PS_DECODE_FP4_STAGES;
 constexpr int kDecodeMaxWarps = kDecodeWarps > kDecodeFp8Warps ? kDecodeWarps : kDecodeFp8Warps;
 constexpr int kDecodeStages = PS_DECODE_STAGES;         // pages in flight per warp
