@@ -35,7 +35,6 @@ constexpr int kFp4Warps = kDecodeFp4Warps;   // streaming warps
 // four pages are what two stages of eight warps leave room for (units of two
 // pages: 161 us where four take 134, before the copying warps).
 constexpr int kFp4UnitPages = 4;
-constexpr int kFp4UnitTokens = kFp4UnitPages * kPageTokens;
 constexpr int kFp4StageBytes = 2 * kFp4UnitPages * kFp4TileBytes;  // K tiles, then V tiles
 static_assert(kFp4UnitPages % 2 == 0, "the scale rows of a unit are copied four tiles at a time");
 static_assert(kFp4StageBytes % 128 == 0, "stage alignment");
