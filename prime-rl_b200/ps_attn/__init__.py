@@ -4,7 +4,8 @@ Modules (imported on demand; nothing is loaded at package import):
 
 * ``ops``       -- torch-facing ops over libps_attn.so: KV append (16-bit and
   fp8), paged decode (split-KV, fused combine and append, cascade, fp8),
-  chunked prefill (tcgen05), fused RoPE + append, the fp8 page gather.
+  chunked prefill (tcgen05), fused RoPE + append, the fp8 page gather; score
+  modifiers (``ScoreMod``) and 4-bit (nvfp4) caches.
 * ``backend``   -- the vLLM attention backend (``register()``).
 * ``sharding``  -- KV-head-sharded decode with the head all-gather over NVLink
   peer memory or NCCL; sequence-batch balancing.

@@ -508,7 +508,8 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
     q/out: [T, Hq, D]; caches [num_blocks, block_size, Hkv, D]; block_table
     int32 [B, P]; seq_lens int32 [B] (including the new token);
     query_start_loc int32 [B+1] or None (row b for sequence b); lse fp32
-    [Hq, T] or None (natural log).
+    [Hq, T] or None (natural log).  Calls that can overlap on the GPU must not
+    share a workspace (the default one is shared by the process).
 
     ``new_key``/``new_value`` [T, Hkv, D] + ``slot_mapping`` int64 [T] fuse the
     KV append of the decode tokens into the same launch (same result as
