@@ -429,8 +429,12 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
     if (fused && cc.p == cc.P - 1 && new_slot >= 0) {
       const int pos = L - 1;
       const int bidx = pos / p.block_size;
-      const int64_t want = static_cast<int64_t>(__ldg(p.block_table + cc.b * p.bt_stride + bidx)) * p.block_size +
-                           (pos - bidx * p.block_size);
+      // (a length past the table, or a slot past the pool, is reported and not stored)
+      const int64_t want =
+          bidx < p.max_blocks_per_seq && new_slot < p.num_blocks * p.block_size
+              ? static_cast<int64_t>(__ldg(p.block_table + cc.b * p.bt_stride + bidx)) * p.block_size +
+                    (pos - bidx * p.block_size)
+              : -1;
       if (new_slot == want) {
         // lanes 0-15: K dims 8c .. 8c + 7, lanes 16-31: V; into this stage's
         // copy of the tile and into the cache, as ps_kv_append_nvfp4 stores them

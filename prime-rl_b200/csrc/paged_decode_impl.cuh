@@ -1071,8 +1071,12 @@ __device__ __forceinline__ int stream_range(const DecodeParams& p, const CUtenso
     if (fused && cc.p == cc.P - 1 && new_slot >= 0) {
       const int pos = L - 1;
       const int bidx = pos / p.block_size;
-      const int64_t want = static_cast<int64_t>(__ldg(p.block_table + cc.b * p.bt_stride + bidx)) *
-                               p.block_size + (pos - bidx * p.block_size);
+      // (a length past the table, or a slot past the pool, is reported and not stored)
+      const int64_t want =
+          bidx < p.max_blocks_per_seq && new_slot < p.num_blocks * p.block_size
+              ? static_cast<int64_t>(__ldg(p.block_table + cc.b * p.bt_stride + bidx)) * p.block_size +
+                    (pos - bidx * p.block_size)
+              : -1;
       if (new_slot == want) {
         // write the row into this stage's copy of the page (K lanes 0-15, V 16-31)
         const int r = pos & (kPageTokens - 1);

@@ -76,7 +76,12 @@ extern "C" int ps_paged_decode_static_scratch(const ps_paged_problem* pr, void* 
   // word and the per-(sequence, kv head) split counters must start at zero:
   // clear them (a completed call leaves the counters at zero, but a call that
   // gave up on a bounded wait may not).
-  const size_t clear = 256 + static_cast<size_t>(pr->num_seqs) * pr->num_kv_heads * 4;
+  size_t clear = 256 + static_cast<size_t>(pr->num_seqs) * pr->num_kv_heads * 4;
+  // a 4-bit cache's decode also counts chunks of splits, two counters per warp
+  // behind the whole counter array
+  if (pr->kv_cache_dtype == PS_KV_NVFP4)
+    clear = 256 + static_cast<size_t>(ps::kDecodeMaxSeqs) * pr->num_kv_heads * 4 +
+            static_cast<size_t>(sms) * ps::kDecodeFp4Warps * 2 * 4;
   if (cudaMemsetAsync(scratch, 0, clear, s) != cudaSuccess) return PS_ERR_CUDA;
   const int rc = ps_paged_decode(pr, scratch, kStaticScratchBytes, stream);
   if (rc != PS_OK) return rc;
