@@ -143,11 +143,15 @@ struct PrefillSmem {
   static constexpr int bytes_before_table = table_off;
 };
 
-// Batches of at most this many sequences list them by falling length when there
+// Batches of at most kOrderSeqs sequences list them by falling length when there
 // are more units than CTAs, so that no CTA starts a long one last (24 follow-up
 // turns of 77 tokens over 129-1,999 cached ones, 192 units: 81 us in batch order,
-// 73 so).  Larger batches have units enough to even out.
+// 72 so).  Past kOrderUnits units for each CTA the tail is a small part, and the
+// plain kernel keeps batch order (four chunks of 1,024 tokens over 3,001-6,001,
+// 512 units: 323 us in it, 326 by falling length); with score modifiers the order
+// stays the better one (packed documents, 243 us against 246).
 constexpr int kOrderSeqs = 128;
+constexpr int kOrderUnits = 2;  // x CTAs
 
 struct PBars {
   uint64_t* q_full;
@@ -219,7 +223,7 @@ __device__ __forceinline__ UnitInfo unit_info(const PrefillParams& p, const int*
   }
   const int npairs = prefix[lo + 1] - prefix[lo];
   const int mp = npairs - 1 - (pu - prefix[lo]);
-  if (order != nullptr) lo = order[lo];
+  if (p.num_seqs <= kOrderSeqs) lo = order[lo];
   ui.b = lo;
   ui.qrow0 = __ldg(p.qsl + lo);
   ui.qlen = __ldg(p.qsl + lo + 1) - ui.qrow0;
@@ -355,6 +359,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int mt = qlen > 0 ? (qlen + tpt - 1) / tpt : 0;
     return (mt + 1) / 2;
   };
+  // (lengths for the order of small batches: read here, beside the pairs)
+  int* order = reinterpret_cast<int*>(smem + L::order_off);
+  const int my_len = B <= kOrderSeqs && tid < B ? __ldg(p.seq_lens + tid) : 0;
   int local = 0;
   for (int b = b_lo; b < b_hi; ++b) local += pairs_of(b);
   int incl = local;
@@ -362,6 +369,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
+  }
+  if (B <= kOrderSeqs && tid < B) {
+    order[tid] = tid;
+    order[kOrderSeqs + tid] = my_len;
   }
   if (lane == 31) s_warp_tot[warp] = incl;
   if (tid == 0) {
@@ -408,32 +419,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   const int total_units = prefix[B] * p.num_kv_heads;
-  int* order = nullptr;
-  if (B > 1 && B <= kOrderSeqs && total_units > static_cast<int>(gridDim.x)) {
-    // rank of each sequence by falling length (ties in batch order), then the
-    // pairs' prefix in that order
-    order = reinterpret_cast<int*>(smem + L::order_off);
-    int* lens = order + kOrderSeqs;
-    const int len = tid < B ? __ldg(p.seq_lens + tid) : 0;
-    if (tid < B) lens[tid] = len;
-    __syncthreads();
-    int rank = 0;
-    for (int b = 0; b < B; ++b) rank += (lens[b] > len || (lens[b] == len && b < tid)) ? 1 : 0;
-    if (tid < B) order[rank] = tid;
-    __syncthreads();
-    if (warp == 0) {
-      int run = 0;
-      for (int r0 = 0; r0 < B; r0 += 32) {
-        const int n = r0 + lane < B ? pairs_of(order[r0 + lane]) : 0;
-        int sum = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += v;
-        }
-        if (r0 + lane < B) prefix[r0 + lane] = run + sum - n;
-        run += __shfl_sync(0xffffffffu, sum, 31);
+  if (B > 1 && B <= kOrderSeqs && total_units > static_cast<int>(gridDim.x) &&
+      (kMod || total_units <= kOrderUnits * static_cast<int>(gridDim.x))) {
+    // each sequence's rank by falling length (ties in batch order) and the pairs
+    // of the sequences before it in that order
+    const int* lens = order + kOrderSeqs;
+    int rank = 0, before = 0;
+#pragma unroll 4
+    for (int b = 0; b < B; ++b) {
+      const int l = lens[b], pairs = prefix[b + 1] - prefix[b];
+      if (l > my_len || (l == my_len && b < tid)) {
+        ++rank;
+        before += pairs;
       }
+    }
+    __syncthreads();  // prefix is read, then rewritten (its last entry stays)
+    if (tid < B) {
+      order[rank] = tid;
+      prefix[rank] = before;
     }
     __syncthreads();
   }

@@ -216,3 +216,14 @@ def test_static_scratch_takes_a_4bit_cache():
         _lib.check(lib.ps_paged_decode_static_scratch(ctypes.byref(pr), torch.cuda.current_stream().cuda_stream))
         mod_ref.check(out, lse, b.reference())
         assert int(status) == 0
+
+
+@pytest.mark.parametrize("m", [None, dict(softcap=30.0, window_left=40)], ids=["plain", "mod"])
+@pytest.mark.parametrize("B,hkv", [(24, 8), (60, 8), (128, 2), (129, 2)])
+def test_prefill_of_many_unequal_sequences(B, hkv, m):
+    """Around the rules that list a batch's sequences by falling length: some without rows, equal lengths, one long."""
+    q_lens = [(i * 5) % 13 for i in range(B)]
+    lens = [q + (i * i * 7) % 90 for i, q in enumerate(q_lens)]
+    lens[B // 2] += 700
+    b = mod_ref.Batch(lens, q_lens, 2 * hkv, hkv, seed=56)
+    mod_ref.check(*run_prefill(b, m), b.reference(m, prefill=True))
