@@ -13,7 +13,7 @@ namespace ps {
 // are, thread t of a page takes page positions 2t, 2t + 1, 2t + 8, 2t + 9: their V
 // words are 16 consecutive bytes of the tile (8 where the tokens straddle two
 // pages), and the two t of a warp fill a 32-byte sector.
-// 16,384 tokens of 8 heads (86 MB): 33 us, 2.6 TB/s -- 19 us of it the rows' loads
+// 16,384 tokens of 8 heads (86 MB): 32 us, 2.7 TB/s -- 19 us of it the rows' loads
 // and their latency, 6 the stores, 8 the quantization.  64 registers (four CTAs per
 // SM) against 79: 33 against 37 us.
 constexpr int kFp4AppendGroup = 16;
@@ -203,7 +203,8 @@ int ps_launch_kv_append_nvfp4(const ps::AppendArgs& a, const float* k_scale, con
                               int dtype_bf16, int sm_count, cudaStream_t stream) {
   if (a.num_tokens == 0) return 0;
   int64_t blocks = (a.num_tokens + ps::kFp4AppendGroup - 1) / ps::kFp4AppendGroup * ((2 * a.num_heads * 64 + 255) / 256);
-  const int64_t cap = static_cast<int64_t>(sm_count) * 8;
+  // (16 CTAs per SM, four of them resident: 32 us for the tokens above, 33 with 8 or 4)
+  const int64_t cap = static_cast<int64_t>(sm_count) * 16;
   if (blocks > cap) blocks = cap;
   if (dtype_bf16)
     ps::kv_append_nvfp4_kernel<true><<<static_cast<int>(blocks), 256, 0, stream>>>(a, k_scale, v_scale);

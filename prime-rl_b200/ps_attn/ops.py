@@ -80,12 +80,12 @@ def is_nvfp4_cache(cache: torch.Tensor, head_size: int = 128) -> bool:
 
 
 def _check_nvfp4(key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
-    if value_cache.dtype != torch.uint8 or key_cache.shape != value_cache.shape or \
-            key_cache.stride() != value_cache.stride():
+    strides = key_cache.stride()
+    if value_cache.dtype != torch.uint8 or key_cache.shape != value_cache.shape or strides != value_cache.stride():
         raise ValueError("nvfp4: key_cache and value_cache must have the same dtype, shape and strides")
     if key_cache.shape[2] % 16:
         raise ValueError("nvfp4: block_size must be a multiple of 16")
-    if key_cache.stride(3) != 1 or key_cache.stride(2) != NVFP4_ROW_BYTES:
+    if strides[3] != 1 or strides[2] != NVFP4_ROW_BYTES:
         raise ValueError("nvfp4: the (block_size, 72) part of a cache must be contiguous")
 
 
@@ -222,17 +222,20 @@ def _append_nvfp4(lib, key, value, key_cache, value_cache, slot_mapping, status,
     _check_nvfp4(key_cache, value_cache)
     if key.dtype != value.dtype or key.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("nvfp4 cache: fp16/bf16 key and value rows of one dtype")
-    if key.stride(-1) != 1 or value.stride(-1) != 1 or not slot_mapping.is_contiguous():
+    k_st, k_sh, k_sd = key.stride()
+    v_st, v_sh, v_sd = value.stride() if value.dim() == 3 else (0, 0, 0)
+    if k_sd != 1 or v_sd != 1 or not slot_mapping.is_contiguous():
         raise ValueError("key/value rows and slot_mapping must be contiguous")
     nb, hkv, bs, _ = key_cache.shape
+    s_block, s_head = key_cache.stride()[:2]
     T = slot_mapping.shape[0]
     if key.shape[0] < T or value.shape[0] < T:
         raise ValueError("key/value have fewer rows than slot_mapping")
     if key.shape[1:] != (hkv, 128) or value.shape[1:] != (hkv, 128):
         raise ValueError(f"key/value shape {tuple(key.shape)} does not match {hkv} kv heads of 128")
     _launch(key.device, lib.ps_kv_append_nvfp4,
-            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
-            key_cache.data_ptr(), value_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1), nb,
+            key.data_ptr(), k_st, k_sh, value.data_ptr(), v_st, v_sh,
+            key_cache.data_ptr(), value_cache.data_ptr(), s_block, s_head, nb,
             slot_mapping.data_ptr(), T, hkv, 128, bs, _DTYPES[key.dtype], _scale_ptr(k_scale),
             _scale_ptr(v_scale), status.data_ptr() if status is not None else None, _stream_ptr(key.device))
 
