@@ -227,3 +227,31 @@ def test_prefill_of_many_unequal_sequences(B, hkv, m):
     lens[B // 2] += 700
     b = mod_ref.Batch(lens, q_lens, 2 * hkv, hkv, seed=56)
     mod_ref.check(*run_prefill(b, m), b.reference(m, prefill=True))
+
+
+@pytest.mark.parametrize("kind", ["16bit", "fp8", "nvfp4"])
+def test_a_bad_query_stays_with_its_row_and_head(kind):
+    """A NaN or infinite query in one head of one row: every other (row, head) as without it."""
+    b = mod_ref.Batch([90, 300, 33], [1] * 3, 8, 2, kind=kind, seed=57)
+    m = dict(softcap=12.0, window_left=120)
+    ref = b.reference(m)
+    keep = torch.ones(3, 8, dtype=torch.bool, device="cuda")
+    b.q = b.q.clone()
+    b.q[1, 2, 5], keep[1, 2] = float("nan"), False
+    b.q[2, 7, 100], keep[2, 7] = float("inf"), False
+    out, lse = run_decode(b, m)
+    for t in range(3):
+        for h in torch.nonzero(keep[t]).flatten().tolist():
+            r = tuple(x[t:t + 1, h:h + 1] if x.dim() == 3 else x[h:h + 1, t:t + 1] for x in ref)
+            mod_ref.check(out[t:t + 1, h:h + 1], lse[h:h + 1, t:t + 1], r)
+
+
+def test_a_bad_query_row_of_a_prompt_stays_with_its_row():
+    b = mod_ref.Batch([300], [300], 8, 2, seed=58)
+    m = dict(softcap=12.0, window_left=120)
+    ref = b.reference(m, prefill=True)
+    b.q = b.q.clone()
+    b.q[140, 3, 9] = float("nan")
+    out, lse = run_prefill(b, m)
+    out[140, 3], lse[3, 140] = ref[0][140, 3].to(out.dtype), ref[1][3, 140].float()
+    mod_ref.check(out, lse, ref)
