@@ -19,7 +19,6 @@ import math
 import torch
 
 own = False
-_imported = None
 
 D = 128        # head size
 PAGE = 16      # tokens of a cache page
@@ -318,24 +317,15 @@ def _plain_attention(st, k, v):
     return [o, lse.permute(0, 3, 1, 2).flatten(2, 3)[st["seq"], at].T.contiguous()]
 
 
-def _ops():
-    """The framework's operators, imported once: a user's program does not look for the package in every call."""
-    global _imported
-    if _imported is None:
-        import sys
-        from pathlib import Path
-
-        here = str(Path(__file__).resolve().parent.parent / "prime-rl_b200")
-        if here not in sys.path:
-            sys.path.insert(0, here)
-        from ps_attn import ops
-
-        _imported = ops
-    return _imported
-
-
 def _own(st):
-    ops = _ops()
+    import sys
+    from pathlib import Path
+
+    here = str(Path(__file__).resolve().parent.parent / "prime-rl_b200")
+    if here not in sys.path:
+        sys.path.insert(0, here)
+    from ps_attn import ops
+
     case = st["case"]
     op = case["op"]
     if op == "store":
