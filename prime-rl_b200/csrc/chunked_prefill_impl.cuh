@@ -887,59 +887,84 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int qh = ui.h * G + hin;
         const int64_t orow = static_cast<int64_t>(ui.qrow0 + tok[x]);
         const uint32_t o_addr = lane_addr + 256 + x * 128 + 64 * half;
-        // Rows are 256 bytes or more apart, so a lane storing its own row's 16-byte
-        // pieces would touch a line per lane.  Four lanes exchange theirs (a 4 x 4
-        // transpose of pieces): a store then fills 64 bytes of eight rows.
-        uint32_t o[2][32];
-        tc::ld_32x32b_x32(o_addr, o[0]);
-        tc::ld_32x32b_x32(o_addr + 32, o[1]);
-        tc::wait_ld();
-        const int q = lane & 3;
-        const int r0 = row - q;
-        uint8_t* dst[4];
-        {
-          int tk = r0 / G, hd = r0 - tk * G;
+        if constexpr (kMod) {
+          // Rows are 256 bytes or more apart, so a lane storing its own row's 16-byte
+          // pieces would touch a line per lane.  Four lanes exchange theirs (a 4 x 4
+          // transpose of pieces): a store then fills 64 bytes of eight rows.  Windows
+          // and documents leave units few tiles to hide stores behind (383 -> 375 us
+          // and 246 -> 238); the plain kernel's units have more, and its tile loop
+          // pays for the registers (8 prompts of 2,048 rows: 886 -> 898 us).
+          uint32_t o[2][32];
+          tc::ld_32x32b_x32(o_addr, o[0]);
+          tc::ld_32x32b_x32(o_addr + 32, o[1]);
+          tc::wait_ld();
+          const int q = lane & 3;
+          const int r0 = row - q;
+          uint8_t* dst[4];
+          {
+            int tk = r0 / G, hd = r0 - tk * G;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int tok_i = ui.t0 + x * tpt + tk;
-            dst[i] = r0 + i < tpt * G && tok_i < ui.qlen
-                         ? reinterpret_cast<uint8_t*>(p.out) +
-                               ((static_cast<int64_t>(ui.qrow0) + tok_i) * p.o_st +
-                                (static_cast<int64_t>(ui.h) * G + hd) * p.o_sh + 64 * half + q * 8) * 2
-                         : nullptr;
-            if (++hd == G) {
-              hd = 0;
-              ++tk;
+            for (int i = 0; i < 4; ++i) {
+              const int tok_i = ui.t0 + x * tpt + tk;
+              dst[i] = r0 + i < tpt * G && tok_i < ui.qlen
+                           ? reinterpret_cast<uint8_t*>(p.out) +
+                                 ((static_cast<int64_t>(ui.qrow0) + tok_i) * p.o_st +
+                                  (static_cast<int64_t>(ui.h) * G + hd) * p.o_sh + 64 * half + q * 8) * 2
+                           : nullptr;
+              if (++hd == G) {
+                hd = 0;
+                ++tk;
+              }
             }
           }
-        }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t v[4][4];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t v[4][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              v[i][k] = pack2<kBF16>(__uint_as_float(o[c][8 * i + 2 * k]) * inv,
-                                     __uint_as_float(o[c][8 * i + 2 * k + 1]) * inv);
+              for (int k = 0; k < 4; ++k)
+                v[i][k] = pack2<kBF16>(__uint_as_float(o[c][8 * i + 2 * k]) * inv,
+                                       __uint_as_float(o[c][8 * i + 2 * k + 1]) * inv);
 #pragma unroll
-          for (int i = 0; i < 4; i += 2)
+            for (int i = 0; i < 4; i += 2)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t got = __shfl_xor_sync(0xffffffffu, q & 1 ? v[i][k] : v[i + 1][k], 1);
-              if (q & 1) v[i][k] = got; else v[i + 1][k] = got;
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, q & 1 ? v[i][k] : v[i + 1][k], 1);
+                if (q & 1) v[i][k] = got; else v[i + 1][k] = got;
+              }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, q & 2 ? v[i][k] : v[i + 2][k], 2);
+                if (q & 2) v[i][k] = got; else v[i + 2][k] = got;
+              }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (dst[i] != nullptr)
+                *reinterpret_cast<uint4*>(dst[i] + c * 64) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t o[32];
+            tc::ld_32x32b_x32(o_addr + c * 32, o);
+            tc::wait_ld();
+            if (row_valid[x]) {
+              uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) +
+                             (orow * p.o_st + static_cast<int64_t>(qh) * p.o_sh + 64 * half + c * 32) * 2;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint4 v;
+                v.x = pack2<kBF16>(__uint_as_float(o[8 * i + 0]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+                v.y = pack2<kBF16>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+                v.z = pack2<kBF16>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+                v.w = pack2<kBF16>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+                *reinterpret_cast<uint4*>(dst + i * 16) = v;
+              }
             }
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t got = __shfl_xor_sync(0xffffffffu, q & 2 ? v[i][k] : v[i + 2][k], 2);
-              if (q & 2) v[i][k] = got; else v[i + 2][k] = got;
-            }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (dst[i] != nullptr)
-              *reinterpret_cast<uint4*>(dst[i] + c * 64) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+          }
         }
         if (half == 0 && valid && p.lse != nullptr)
           p.lse[static_cast<int64_t>(qh) * p.lse_sh + orow * p.lse_st] =
