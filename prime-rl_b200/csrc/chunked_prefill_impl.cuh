@@ -144,14 +144,14 @@ struct PrefillSmem {
 };
 
 // Batches of at most kOrderSeqs sequences list them by falling length when there
-// are more units than CTAs, so that no CTA starts a long one last (24 follow-up
-// turns of 77 tokens over 129-1,999 cached ones, 192 units: 81 us in batch order,
-// 72 so).  Past kOrderUnits units for each CTA the tail is a small part, and the
-// plain kernel keeps batch order (four chunks of 1,024 tokens over 3,001-6,001,
-// 512 units: 323 us in it, 326 by falling length); with score modifiers the order
-// stays the better one (packed documents, 243 us against 246).
+// are more units than CTAs, so that no CTA starts a long one last.  Batch order
+// against this one, 8 to 32 heads over 1 to 8: 24 follow-up turns of 77 tokens
+// over 129-1,999 cached ones, 192 units, 73 -> 58 us; 24 prompts, 680 units, 154 -> 119;
+// 90 prompts, 1,229 units, 265 -> 211; 4 chunks of 1,024 over 3,001-6,001, 512 units,
+// 380 -> 373; 8 prompts of 2,048 rows, 2,048 units, 990 -> 976.  Of 70 batches of 6 to
+// 90 sequences and 160 to 1,520 units the worst were 6 sequences in 943 units,
+// 498 -> 512, and in 560, 74.7 -> 76.0.
 constexpr int kOrderSeqs = 128;
-constexpr int kOrderUnits = 2;  // x CTAs
 
 struct PBars {
   uint64_t* q_full;
@@ -419,8 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   const int total_units = prefix[B] * p.num_kv_heads;
-  if (B > 1 && B <= kOrderSeqs && total_units > static_cast<int>(gridDim.x) &&
-      (kMod || total_units <= kOrderUnits * static_cast<int>(gridDim.x))) {
+  if (B > 1 && B <= kOrderSeqs && total_units > static_cast<int>(gridDim.x)) {
     // each sequence's rank by falling length (ties in batch order) and the pairs
     // of the sequences before it in that order
     const int* lens = order + kOrderSeqs;
