@@ -516,13 +516,13 @@ __device__ __forceinline__ void stream_range_fp4(const DecodeParams& p, const Ta
           if (p.mod.cap_log2 > 0.f) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              s[u][nt][c] = mod_score<true>(p.mod, s[u][nt][c] * sc[nt][c & 1], scale_log2, k_scale,
-                                            slope[nt][c & 1], c < 2 ? d0 : d1);
+              s[u][nt][c] = mod_score<true>(p.mod, s[u][nt][c] * sc[nt][c & 1], scale_log2, slope[nt][c & 1],
+                                            c < 2 ? d0 : d1);
           } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              s[u][nt][c] = mod_score<false>(p.mod, s[u][nt][c] * sc[nt][c & 1], scale_log2, k_scale,
-                                             slope[nt][c & 1], c < 2 ? d0 : d1);
+              s[u][nt][c] = mod_score<false>(p.mod, s[u][nt][c] * sc[nt][c & 1], scale_log2, slope[nt][c & 1],
+                                             c < 2 ? d0 : d1);
           }
         } else {
 #pragma unroll

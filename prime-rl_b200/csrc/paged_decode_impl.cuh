@@ -155,18 +155,26 @@ __device__ __forceinline__ int mod_skip_pages(const DecodeParams& p, int b, int 
   const int L = __ldg(p.seq_lens + b);
   return max(0, max(0, min(mod_key_low(p, b, L), L - 1)) / kPageTokens - pg0);
 }
+// c tanh(z / c) of a score z in the exp2 domain (c = cap_log2).  Each score takes
+// the form that is accurate for it, whatever the others in its tile:
+//   |z| <= c / 2: z + z t P(t) with t = (z / c)^2 and P a cubic (minimax for
+//     tanh(u) = u + u t P(t), 1.5e-8) -- it tends to z as the cap grows;
+//   beyond:       c - 2c / (1 + exp(2 z / c)), whose error (2^-22 c) would not
+//     shrink with z: at a cap of 1e6 scores near 1 would be 0.09 off.
+// (The hardware tanh's 2^-11 is too coarse for either.)
+__device__ __forceinline__ float mod_cap(const ScoreModParams& m, float z) {
+  const float u = z * m.cap_inv, t = u * u;
+  const float near = fmaf(z * t, fmaf(fmaf(fmaf(0.017241478f, t, -0.05304549f), t, 0.13325879f), t, -0.33333144f), z);
+  const float far = fmaf(-2.f * m.cap_log2, __fdividef(1.f, 1.f + ex2(u * 2.8853900817779268f)), m.cap_log2);
+  return fabsf(u) <= 0.5f ? near : far;
+}
 // Score of one key in the exp2 domain before masking: x is the raw dot
-// product.  Cap: c tanh(z / c) = c - 2c / (1 + exp(2 z / c)) -- exp and
-// reciprocal errors (2^-22) stay absolute in units of c, unlike the hardware
-// tanh's 2^-11.  Bias: slope * (j - i), `dist` = j - i.
+// product.  Bias: slope * (j - i), `dist` = j - i.
 template <bool kCapped>
-__device__ __forceinline__ float mod_score(const ScoreModParams& m, float x, float scale_log2, float k_scale,
-                                           float slope_log2, float dist) {
-  float y;
-  if constexpr (kCapped)
-    y = fmaf(-2.f * m.cap_log2, __fdividef(1.f, 1.f + ex2(x * (m.cap_in * k_scale))), m.cap_log2);
-  else
-    y = x * scale_log2;
+__device__ __forceinline__ float mod_score(const ScoreModParams& m, float x, float scale_log2, float slope_log2,
+                                           float dist) {
+  float y = x * scale_log2;
+  if constexpr (kCapped) y = mod_cap(m, y);
   return fmaf(slope_log2, dist, y);
 }
 
@@ -1163,13 +1171,11 @@ __device__ __forceinline__ int stream_range(const DecodeParams& p, const CUtenso
           if (p.mod.cap_log2 > 0.f) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              s[u][nt][c] = mod_score<true>(p.mod, s[u][nt][c], scale_log2, k_scale, slope[nt][c & 1],
-                                            c < 2 ? d0 : d1);
+              s[u][nt][c] = mod_score<true>(p.mod, s[u][nt][c], scale_log2, slope[nt][c & 1], c < 2 ? d0 : d1);
           } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              s[u][nt][c] = mod_score<false>(p.mod, s[u][nt][c], scale_log2, k_scale, slope[nt][c & 1],
-                                             c < 2 ? d0 : d1);
+              s[u][nt][c] = mod_score<false>(p.mod, s[u][nt][c], scale_log2, slope[nt][c & 1], c < 2 ? d0 : d1);
           }
           if (!v0) s[u][nt][0] = s[u][nt][1] = -INFINITY;
           if (!v1) s[u][nt][2] = s[u][nt][3] = -INFINITY;

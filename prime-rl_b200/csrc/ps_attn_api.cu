@@ -173,6 +173,7 @@ int score_mod_params(const ps_score_mod* m, float scale, ps::ScoreModParams* out
   *out = {};
   if (m->logits_soft_cap > 0.f) {
     out->cap_log2 = m->logits_soft_cap * log2e;
+    out->cap_inv = 1.f / out->cap_log2;
     out->cap_in = 2.f * log2e * scale / m->logits_soft_cap;
     // (a cap whose constants leave fp32's normal range would turn scores into NaN)
     if (!(out->cap_log2 >= 1.2e-38f) || !(out->cap_log2 <= 1.7e38f) || !(out->cap_in <= 3.4e38f))

@@ -27,6 +27,7 @@ struct AppendArgs {
 // Score modifiers of an attention call, derived from ps_score_mod.
 struct ScoreModParams {
   float cap_log2;            // cap * log2(e); 0: no cap
+  float cap_inv;             // 1 / cap_log2
   float cap_in;              // 2 * log2(e) * softmax_scale / cap
   const float* slopes;       // [num_q_heads] bias slopes; nullptr: none
   int32_t window_left;       // keys j >= i - window_left; < 0: no window
