@@ -608,9 +608,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float cap2 = kCap ? p.mod.cap_log2 : 0.f;
     const float cap_in = kCap ? p.mod.cap_in * (p.k_scale ? __ldg(p.k_scale) : 1.f) : 0.f;
     // z / cap = cap_u * raw score; a warp whose scores stay within cap_fast
-    // (|z| <= cap / 2) takes the polynomial
+    // (|z| <= cap / 2) takes the polynomial.  No score does where its
+    // coefficients, which go with cap_u^6, could overflow: not even one of zero.
     const float cap_u = cap_in * 0.34657359f;
-    const float cap_fast = cap_u <= 1e4f ? 0.5f / cap_u : 0.f;
+    const float cap_fast = cap_u <= 1e4f ? 0.5f / cap_u : -1.f;
     for (int u = blockIdx.x; u < total_units; ++uit) {
       UnitInfo ui = unit_info(p, prefix, order, u);
       if constexpr (kMod) mod_unit_range(p, ui, lane);

@@ -72,6 +72,15 @@ def test_decode_caps_of_every_size(kind, dtype, cap):
     mod_ref.check(*run_decode(b, dict(softcap=cap)), capped(b, cap, False))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cap", CAPS)
+def test_prefill_caps_of_every_size(dtype, cap):
+    b = mod_ref.Batch([1, 2, 65, 300], [1, 2, 30, 300], 8, 2, dtype=dtype, seed=73, spread=2.0)
+    b.q[1] = 0  # scores of exactly zero, in a warp with others and in warps of their own
+    b.q[-150:] = 0
+    mod_ref.check(*run_prefill(b, dict(softcap=cap)), capped(b, cap, True))
+
+
 def one_far_key(kind, cap, qlens, lens):
     """Every sequence's key 5 is far below or above the others for every head of kv head 0 and 1: z of about -0.8
     and 0.8 cap, in the reach of the exponential form, beside ordinary scores."""
