@@ -604,14 +604,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float sl2 = p.scale_log2 * (p.k_scale ? __ldg(p.k_scale) : 1.f);
     const float v_scale = p.v_scale ? __ldg(p.v_scale) : 1.f;
     int t = 0, uit = 0;
-    // score modifiers: cap constants in the exp2 domain
+    // Tanh cap, c = cap2 in the exp2 domain: z / c = cap_u * raw score.  A warp whose
+    // scores stay within cap_fast takes the polynomial: |z| <= c / 2, or less where
+    // cap_u's sixth power, in its last coefficient, leaves fp32's range -- z up to
+    // 2^-13 c, of which nothing but the first counts, or none.
     const float cap2 = kCap ? p.mod.cap_log2 : 0.f;
-    const float cap_in = kCap ? p.mod.cap_in * (p.k_scale ? __ldg(p.k_scale) : 1.f) : 0.f;
-    // z / cap = cap_u * raw score; a warp whose scores stay within cap_fast
-    // (|z| <= cap / 2) takes the polynomial.  No score does where its
-    // coefficients, which go with cap_u^6, could overflow: not even one of zero.
-    const float cap_u = cap_in * 0.34657359f;
-    const float cap_fast = cap_u <= 1e4f ? 0.5f / cap_u : -1.f;
+    const float cap_u = kCap ? fminf(sl2 * p.mod.cap_inv, 3.0e38f) : 0.f;
+    const float cap_fast = cap_u < 0x1p-15f ? fminf(0x1p-13f / cap_u, 1e18f) : cap_u <= 0x1p15f ? 0.49999f / cap_u : -1.f;
     for (int u = blockIdx.x; u < total_units; ++uit) {
       UnitInfo ui = unit_info(p, prefix, order, u);
       if constexpr (kMod) mod_unit_range(p, ui, lane);
@@ -662,9 +661,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             // (minimax, relative error 5.4e-7): five packed instructions for two
             // scores on the FMA pipe, where exp and reciprocal take four turns
             // of the MUFU unit, which sets the pace of a tile.  Window and cap on
-            // 13,000 prompt tokens, 32 / 8 heads: 386 us, 493 with the
-            // exponential for every score, 296 without a cap.  (A quadratic for
-            // z up to c / 4: 383.)
+            // 13,000 prompt tokens, 32 / 8 heads: 391 us, 493 with the
+            // exponential for every score, 285 without a cap.  (A quadratic for
+            // z up to c / 4 gained 1 %.)  A warp with a score beyond takes both
+            // forms and each score its own, so that what a score becomes depends on
+            // nothing else: not on the row's other scores (the exponential's error,
+            // 2^-22 c, is too much for small ones), nor on what lies in keys that no
+            // row sees.  (Registers for that: 14 of the 391 us.)
             float am[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -673,10 +676,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 am[i & 3] = max3(am[i & 3], fabsf(__uint_as_float(r[c][2 * i])), fabsf(__uint_as_float(r[c][2 * i + 1])));
             // (a NaN, in keys past the range or not, stays a NaN either way)
             const float amax = fmaxf(max3(am[0], am[1], am[2]), am[3]);
-            const float a2 = cap_u * cap_u, a1 = cap2 * cap_u;
             if (__all_sync(0xffffffffu, amax <= cap_fast)) {
-              const float k0 = a1 * 0.99999946f, k1 = -0.3332632f * a1 * a2;
-              const float k2 = 0.13190296f * a1 * a2 * a2, k3 = -0.044402227f * a1 * a2 * a2 * a2;
+              const float a2 = cap_u * cap_u, k0 = sl2 * 0.99999946f, k1 = -0.3332632f * (sl2 * a2);
+              const float k2 = 0.13190296f * (sl2 * a2) * a2, k3 = -0.044402227f * (sl2 * a2) * a2 * a2;
               const uint64_t q0 = f2_pack(k0, k0), q1 = f2_pack(k1, k1), q2 = f2_pack(k2, k2), q3 = f2_pack(k3, k3);
 #pragma unroll
               for (int c = 0; c < 2; ++c)
@@ -690,12 +692,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                   r[c][2 * i + 1] = __float_as_uint(y1);
                 }
             } else {
+              // the same polynomial in w = raw score * 2^n, z / c = cap_r w with
+              // cap_r in [1/2, 1) (bit for bit what the other branch computes)
+              const int e = min(max((__float_as_int(cap_u) >> 23) + 1, 27), 253);
+              const float s = __int_as_float(e << 23), inv_s = __int_as_float((254 - e) << 23);
+              const float cap_r = cap_u * inv_s, cap_k = sl2 * inv_s, a2 = cap_r * cap_r;
+              const float far_in = cap_r * 2.8853900817779268f;
+              const float k0 = cap_k * 0.99999946f, k1 = -0.3332632f * (cap_k * a2);
+              const float k2 = 0.13190296f * (cap_k * a2) * a2, k3 = -0.044402227f * (cap_k * a2) * a2 * a2;
+              const uint64_t q0 = f2_pack(k0, k0), q1 = f2_pack(k1, k1), q2 = f2_pack(k2, k2), q3 = f2_pack(k3, k3);
 #pragma unroll
               for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int i = 0; i < 32; ++i)  // c tanh(z / c) = c - 2c / (1 + exp(2 z / c))
-                  r[c][i] = __float_as_uint(fmaf(
-                      -2.f * cap2, __fdividef(1.f, 1.f + ex2(__uint_as_float(r[c][i]) * cap_in)), cap2));
+                for (int i = 0; i < 16; ++i) {
+                  const float w0 = __uint_as_float(r[c][2 * i]) * s, w1 = __uint_as_float(r[c][2 * i + 1]) * s;
+                  const uint64_t w = f2_pack(w0, w1);
+                  const uint64_t w2 = f2_mul(w, w);
+                  float y0, y1;
+                  f2_unpack(f2_mul(w, f2_fma(f2_fma(f2_fma(q3, w2, q2), w2, q1), w2, q0)), y0, y1);
+                  // c tanh(z / c) = c - 2c / (1 + exp(2 z / c)); a NaN stays one
+                  const float f0 = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + ex2(w0 * far_in)), cap2);
+                  const float f1 = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + ex2(w1 * far_in)), cap2);
+                  r[c][2 * i] = __float_as_uint(fabsf(w0) * cap_r <= 0.5f ? y0 : f0);
+                  r[c][2 * i + 1] = __float_as_uint(fabsf(w1) * cap_r <= 0.5f ? y1 : f1);
+                }
             }
           }
           if constexpr (kBias) {

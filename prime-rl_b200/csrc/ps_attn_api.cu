@@ -162,8 +162,8 @@ int validate_nvfp4_strides(const ps_paged_problem* pr) {
   return PS_OK;
 }
 
-// ps_score_mod -> kernel parameters.  scale: the problem's softmax_scale.
-int score_mod_params(const ps_score_mod* m, float scale, ps::ScoreModParams* out) {
+// ps_score_mod -> kernel parameters.
+int score_mod_params(const ps_score_mod* m, ps::ScoreModParams* out) {
   if (!m) return fail(PS_ERR_INVALID_ARGUMENT, "score modifiers are NULL");
   if (!(m->logits_soft_cap >= 0.f) || !(m->logits_soft_cap <= 3.0e38f))
     return fail(PS_ERR_INVALID_ARGUMENT, "logits_soft_cap must be finite and >= 0 (0: no cap)");
@@ -174,9 +174,8 @@ int score_mod_params(const ps_score_mod* m, float scale, ps::ScoreModParams* out
   if (m->logits_soft_cap > 0.f) {
     out->cap_log2 = m->logits_soft_cap * log2e;
     out->cap_inv = 1.f / out->cap_log2;
-    out->cap_in = 2.f * log2e * scale / m->logits_soft_cap;
     // (a cap whose constants leave fp32's normal range would turn scores into NaN)
-    if (!(out->cap_log2 >= 1.2e-38f) || !(out->cap_log2 <= 1.7e38f) || !(out->cap_in <= 3.4e38f))
+    if (!(out->cap_log2 >= 1.2e-38f) || !(out->cap_log2 <= 1.7e38f))
       return fail(PS_ERR_INVALID_ARGUMENT, "logits_soft_cap %g is outside the usable range",
                   static_cast<double>(m->logits_soft_cap));
   }
@@ -245,7 +244,7 @@ int decode_impl(const ps_paged_problem* pr, const void* plan, int64_t plan_bytes
   if (rc != PS_OK) return rc;
   ps::ScoreModParams modp = {};
   if (mod != nullptr) {
-    rc = score_mod_params(mod, pr->softmax_scale, &modp);
+    rc = score_mod_params(mod, &modp);
     if (rc != PS_OK) return rc;
   }
   if (pr->num_seqs == 0) return PS_OK;
@@ -727,7 +726,7 @@ int prefill_impl(const ps_paged_problem* pr, void* workspace, int64_t workspace_
     return fail(PS_ERR_UNSUPPORTED, "chunked prefill over an fp8 cache is not built");
   ps::ScoreModParams modp = {};
   if (mod != nullptr) {
-    rc = score_mod_params(mod, pr->softmax_scale, &modp);
+    rc = score_mod_params(mod, &modp);
     if (rc != PS_OK) return rc;
   }
   if (pr->num_seqs == 0 || pr->num_tokens == 0) return PS_OK;

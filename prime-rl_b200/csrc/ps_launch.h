@@ -28,7 +28,6 @@ struct AppendArgs {
 struct ScoreModParams {
   float cap_log2;            // cap * log2(e); 0: no cap
   float cap_inv;             // 1 / cap_log2
-  float cap_in;              // 2 * log2(e) * softmax_scale / cap
   const float* slopes;       // [num_q_heads] bias slopes; nullptr: none
   int32_t window_left;       // keys j >= i - window_left; < 0: no window
   const int32_t* key_start;  // [query rows] first key of the row's document; nullptr: 0

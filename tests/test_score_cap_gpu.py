@@ -106,3 +106,32 @@ def test_decode_one_far_key(kind, cap):
     """A score far beyond c / 2 leaves the accuracy of the others in its tile alone."""
     b = one_far_key(kind, cap, [1, 1, 1], [40, 50, 300])
     mod_ref.check(*run_decode(b, dict(softcap=cap)), capped(b, cap, False))
+
+
+@pytest.mark.parametrize("cap", [1e3, 1e4])
+def test_prefill_one_far_key(cap):
+    b = one_far_key("16bit", cap, [40, 40, 40], [40, 50, 300])
+    mod_ref.check(*run_prefill(b, dict(softcap=cap)), capped(b, cap, True))
+
+
+@pytest.mark.parametrize("window", [None, 40])
+def test_prefill_bits_do_not_depend_on_keys_nobody_sees(window):
+    """Slots past a sequence, keys below its window and unused blocks hold NaN, then small, then huge values; more
+    units than CTAs, handed out dynamically or in turn: the same bits each time."""
+    lens = [5 + (i * 29) % 150 for i in range(40)]
+    b = mod_ref.Batch(lens, [min(n, 3 + i % 50) for i, n in enumerate(lens)], 16, 8, seed=74, spread=2.0)
+    m = dict(softcap=9.0) if window is None else dict(softcap=9.0, window_left=window)
+    unused = torch.isnan(b.kc)
+    if window is not None:  # keys that no row of their sequence sees
+        row = 0
+        for i, n in enumerate(lens):
+            for slot in b.slots[row:row + max(0, n - b.qlens[i] - window)].tolist():
+                unused[slot // b.bs, slot % b.bs] = True
+            row += n
+    first = run_prefill(b, m)
+    for value in (0.01, 3e38, -3e38):
+        b.kc, b.vc = b.kc.masked_fill(unused, value), b.vc.masked_fill(unused, value)
+        for ws in (True, False, True):
+            again = run_prefill(b, m, workspace=ws)
+            assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+    mod_ref.check(*first, capped(b, 9.0, True, window))
