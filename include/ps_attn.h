@@ -58,6 +58,11 @@ typedef enum { PS_DTYPE_FP16 = 0, PS_DTYPE_BF16 = 1, PS_DTYPE_FP32 = 2 } ps_dtyp
 int ps_abi_version(void);
 const char* ps_last_error(void);
 
+/* The identity of the CUDA-graph capture that `stream` is in (unique in the
+ * process), 0 if it is in none: for callers that keep workspaces and must not
+ * share one between graphs that can run at the same time. */
+uint64_t ps_stream_capture_id(void* stream);
+
 /*
  * KV append.  Replaces torch.ops._C_cache_ops.reshape_and_cache_flash
  * (vllm/_custom_ops.py:2591-2610; semantics of its readable twin

@@ -389,6 +389,16 @@ int ps_abi_version(void) { return PS_ATTN_ABI_VERSION; }
 
 const char* ps_last_error(void) { return g_err; }
 
+uint64_t ps_stream_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
 int ps_kv_append(const void* key, int64_t key_stride_token, int64_t key_stride_head,
                  const void* value, int64_t value_stride_token, int64_t value_stride_head,
                  void* key_cache, void* value_cache, int64_t cache_stride_block,

@@ -70,6 +70,7 @@ EXPORTED_SYMBOLS = (
     "ps_kv_append_nvfp4",
     "ps_paged_decode_mod",
     "ps_chunked_prefill_mod",
+    "ps_stream_capture_id",
 )
 PS_HEAD_GATHER_ROWS_OFFSET = 256
 
@@ -250,6 +251,8 @@ def _declare(lib):
         c.c_void_p, c.c_int64, c.c_int, c.c_int, c.c_int, c.c_int,  # slots, shape
         c.c_void_p, c.c_void_p,  # status, stream
     ]
+    lib.ps_stream_capture_id.restype = c.c_uint64
+    lib.ps_stream_capture_id.argtypes = [c.c_void_p]
     lib.ps_kv_append_nvfp4.restype = c.c_int
     lib.ps_kv_append_nvfp4.argtypes = [
         c.c_void_p, c.c_int64, c.c_int64, c.c_void_p, c.c_int64, c.c_int64, c.c_void_p, c.c_void_p,

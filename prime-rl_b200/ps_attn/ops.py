@@ -343,20 +343,36 @@ class DecodeWorkspace:
         self.buffer[:4].zero_()
 
 
-_WS_CACHE: dict = {}
+_WS_CACHE: dict = {}       # (device, stream, heads, kind) -> workspace of the stream's own calls
+_WS_CAPTURES: dict = {}    # (device, stream) -> (capture, {(heads, kind): workspace}) of the stream's last capture
 
 
 def get_workspace(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_size: int,
                   device: torch.device, cascade: bool = False) -> DecodeWorkspace:
-    """Process-wide workspace per (device, heads, kind), grown to the largest batch seen."""
-    key = (device.index, num_q_heads, num_kv_heads, head_size, cascade)
-    ws = _WS_CACHE.get(key)
+    """The workspace of calls on ``device``'s current stream, per (heads, kind), grown to the largest batch seen.
+
+    Calls of one stream run one after the other, so they can share it.  A call
+    that is captured into a CUDA graph gets a workspace of that graph's: it lives
+    in the graph's memory pool and is zeroed by each replay, so that neither a
+    larger batch later on, nor another graph, nor the stream's own calls touch it."""
+    lib = _lib.load()
+    stream = _stream_ptr(device)
+    key = (num_q_heads, num_kv_heads, head_size, cascade)
+    capture = lib.ps_stream_capture_id(stream)
+    if capture:
+        of, kept = _WS_CAPTURES.get((device.index, stream), (0, None))
+        if of != capture:
+            kept = {}
+            _WS_CAPTURES[device.index, stream] = (capture, kept)
+    else:
+        kept, key = _WS_CACHE, (device.index, stream) + key
+    ws = kept.get(key)
     if ws is None or ws.max_num_seqs < num_seqs:
         cap = max(num_seqs, 256 if ws is None else 2 * ws.max_num_seqs)
         if cascade:
             cap = min(cap, CASCADE_MAX_SEQS)
         ws = DecodeWorkspace(cap, num_q_heads, num_kv_heads, head_size, device, cascade=cascade)
-        _WS_CACHE[key] = ws
+        kept[key] = ws
     return ws
 
 
@@ -512,7 +528,8 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
     int32 [B, P]; seq_lens int32 [B] (including the new token);
     query_start_loc int32 [B+1] or None (row b for sequence b); lse fp32
     [Hq, T] or None (natural log).  Calls that can overlap on the GPU must not
-    share a workspace (the default one is shared by the process).
+    share a workspace (the default one is shared by the calls of a stream, or of a
+    captured graph: :func:`get_workspace`).
 
     ``new_key``/``new_value`` [T, Hkv, D] + ``slot_mapping`` int64 [T] fuse the
     KV append of the decode tokens into the same launch (same result as
