@@ -220,6 +220,8 @@ int ps_kv_dequant_gather(const ps_paged_problem* problem, int32_t max_pages, voi
  * buffer sized for max_num_seqs serves every step and every CUDA-graph
  * replay.  The buffer must be zeroed once before first use (the kernel keeps
  * its counters at zero between calls); its first int32 is the status word.
+ * It serves calls with one num_kv_heads (of any group): the counters' place
+ * depends on it, so zero the buffer again before calls with another.
  * After PS_DEV_WAIT_TIMEOUT the buffer must be zeroed again.
  */
 int64_t ps_paged_decode_workspace_size(int32_t num_seqs, int32_t num_q_heads,

@@ -311,7 +311,8 @@ class DecodeWorkspace:
 
     Sized for ``max_num_seqs`` once (independent of sequence lengths, so one
     buffer serves every step and every CUDA-graph replay) and zeroed at
-    creation; the kernel leaves its counters at zero.  ``status()`` reads and
+    creation; the kernel leaves its counters at zero.  Serves calls with
+    ``num_kv_heads`` kv heads only: the counters' place depends on them.  ``status()`` reads and
     ``clear_status()`` resets the device status word (PS_DEV_* bits).
     """
 
@@ -567,11 +568,14 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
     fp4 = is_nvfp4_cache(key_cache, q.shape[-1])
     if (fp4 or score_mod is not None) and (cascade is not None or head_gather is not None):
         raise ValueError("nvfp4 caches and score modifiers take neither a cascade plan nor the fused head gather")
+    hkv, d = (key_cache.shape[1], q.shape[2]) if fp4 else (key_cache.shape[2], key_cache.shape[3])
     if workspace is None:
-        hkv, d = (key_cache.shape[1], q.shape[2]) if fp4 else (key_cache.shape[2], key_cache.shape[3])
         workspace = get_workspace(B, q.shape[1], hkv, d, q.device, cascade=cascade is not None)
     elif workspace.max_num_seqs < B:
         raise ValueError(f"workspace sized for {workspace.max_num_seqs} sequences < {B}")
+    elif workspace.num_kv_heads not in (None, hkv):
+        # partial rows of one head count would lie on the counters of another
+        raise ValueError(f"workspace made for {workspace.num_kv_heads} kv heads, the call has {hkv}")
     if cascade is not None and cascade.num_seqs != B:
         raise ValueError(f"cascade plan built for {cascade.num_seqs} sequences, call has {B}")
     pr = _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
@@ -589,7 +593,6 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
             raise ValueError("slot_mapping must be contiguous int64")
         if new_key.dtype != q.dtype or new_value.dtype != q.dtype:
             raise ValueError("new key/value must have the query dtype")
-        hkv, d = (key_cache.shape[1], q.shape[2]) if fp4 else (key_cache.shape[2], key_cache.shape[3])
         if new_key.shape[1:] != (hkv, d) or new_value.shape[1:] != (hkv, d):
             raise ValueError("new key/value shape does not match the cache")
         if new_key.stride(-1) != 1 or new_value.stride(-1) != 1:

@@ -22,8 +22,8 @@ implementation (shape-only, no launch) for tracing:
   and cache scales; the decode takes 16-bit, fp8 and nvfp4 caches.
 
 Conventions of the C ABI hold: caller-allocated outputs and workspace (a
-``uint8`` tensor of ``DecodeWorkspace``'s size, zeroed once), the current
-CUDA stream, no host synchronisation, errors raised as
+``uint8`` tensor of ``DecodeWorkspace``'s size, zeroed once, for calls with one
+number of kv heads), the current CUDA stream, no host synchronisation, errors raised as
 :class:`ps_attn._lib.PSError`.  ``max_seq_len`` is accepted for signature
 parity with vLLM's call and not needed by the kernels.  vLLM's attention
 layer already wraps the backend in its own opaque custom op
@@ -50,6 +50,7 @@ class _WorkspaceView:
         self.buffer = buffer
         self.nbytes = buffer.numel()
         self.max_num_seqs = num_seqs
+        self.num_kv_heads = None  # (a tensor does not say whose it is)
 
 
 @torch.library.custom_op("ps_attn::kv_append", mutates_args=("key_cache", "value_cache"))

@@ -76,3 +76,21 @@ def test_a_first_call_inside_a_capture_leaves_nothing_behind(fakes):
     captured = get()
     fakes.capture = 0
     assert get() is not captured
+
+
+@pytest.mark.parametrize("cache", ["16bit", "nvfp4"])
+def test_a_workspace_of_another_head_count_is_refused(cache):
+    """Its counters lie where calls with this many heads put partial rows."""
+    class Workspace:
+        max_num_seqs, num_q_heads, num_kv_heads = 8, 16, 8
+
+    q = torch.zeros(2, 16, 128, dtype=torch.bfloat16)
+    kc = torch.zeros(4, 16, 2, 128, dtype=torch.bfloat16)
+    if cache == "nvfp4":
+        kc = torch.zeros(ops.nvfp4_cache_shape(4, 16, 2), dtype=torch.uint8)
+    table, lens = torch.zeros(2, 4, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="8 kv heads, the call has 2"):
+        ops.paged_decode(q, kc, kc, table, lens, 0.1, q, workspace=Workspace())
+    Workspace.num_kv_heads = 2
+    with pytest.raises(ValueError, match="CUDA"):  # past the workspace's checks
+        ops.paged_decode(q, kc, kc, table, lens, 0.1, q, workspace=Workspace())
