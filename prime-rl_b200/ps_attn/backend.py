@@ -398,9 +398,12 @@ class PSScoreModAttentionImpl(PSAttentionImpl):
 
     def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int,
                  alibi_slopes: list[float] | None = None, sliding_window: int | None = None,
-                 kv_cache_dtype: str = "auto", logits_soft_cap: float | None = None, **kwargs) -> None:
+                 kv_cache_dtype: str = "auto", logits_soft_cap: float | None = None,
+                 attn_type: str = AttentionType.DECODER,
+                 kv_sharing_target_layer_name: str | None = None,
+                 sinks: torch.Tensor | None = None) -> None:
         super().__init__(num_heads, head_size, scale, num_kv_heads, alibi_slopes, sliding_window,
-                         kv_cache_dtype, logits_soft_cap, **kwargs)
+                         kv_cache_dtype, logits_soft_cap, attn_type, kv_sharing_target_layer_name, sinks)
         if self.dcp:
             raise NotImplementedError("decode context parallelism with score modifiers is not supported")
         if sliding_window is not None and sliding_window < 1:
