@@ -198,24 +198,24 @@ def kv_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
     if key.shape[1:] != (hkv, d) or value.shape[1:] != (hkv, d):
         raise ValueError(f"key/value shape {tuple(key.shape)} does not match cache {tuple(key_cache.shape)}")
     if fp8:
-        _lib.check(lib.ps_kv_append_fp8(
+        _launch(key.device, lib.ps_kv_append_fp8,
+                key.data_ptr(), key.stride(0), key.stride(1),
+                value.data_ptr(), value.stride(0), value.stride(1),
+                key_cache.data_ptr(), value_cache.data_ptr(),
+                key_cache.stride(0), key_cache.stride(1), key_cache.stride(2), nb,
+                slot_mapping.data_ptr(), T, hkv, d, bs, _DTYPES[key.dtype],
+                _scale_ptr(k_scale), _scale_ptr(v_scale),
+                status.data_ptr() if status is not None else None,
+                _stream_ptr(key.device))
+        return
+    _launch(key.device, lib.ps_kv_append,
             key.data_ptr(), key.stride(0), key.stride(1),
             value.data_ptr(), value.stride(0), value.stride(1),
             key_cache.data_ptr(), value_cache.data_ptr(),
             key_cache.stride(0), key_cache.stride(1), key_cache.stride(2), nb,
-            slot_mapping.data_ptr(), T, hkv, d, bs, _DTYPES[key.dtype],
-            _scale_ptr(k_scale), _scale_ptr(v_scale),
+            slot_mapping.data_ptr(), T, hkv, d, bs, key.element_size(),
             status.data_ptr() if status is not None else None,
-            _stream_ptr(key.device)))
-        return
-    _lib.check(lib.ps_kv_append(
-        key.data_ptr(), key.stride(0), key.stride(1),
-        value.data_ptr(), value.stride(0), value.stride(1),
-        key_cache.data_ptr(), value_cache.data_ptr(),
-        key_cache.stride(0), key_cache.stride(1), key_cache.stride(2), nb,
-        slot_mapping.data_ptr(), T, hkv, d, bs, key.element_size(),
-        status.data_ptr() if status is not None else None,
-        _stream_ptr(key.device)))
+            _stream_ptr(key.device))
 
 
 def _append_nvfp4(lib, key, value, key_cache, value_cache, slot_mapping, status, k_scale, v_scale) -> None:
@@ -303,7 +303,7 @@ def rope_kv_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     pr.dtype = _DTYPES[dtype]
     if status is not None:
         pr.status = status.data_ptr()
-    _lib.check(lib.ps_rope_kv_append(ctypes.byref(pr), _stream_ptr(query.device)))
+    _launch(query.device, lib.ps_rope_kv_append, ctypes.byref(pr), _stream_ptr(query.device))
 
 
 class DecodeWorkspace:
@@ -449,9 +449,8 @@ def cascade_plan(block_table: torch.Tensor, seq_lens: torch.Tensor, num_q_heads:
     pr.num_kv_heads = num_kv_heads
     pr.head_size = 128
     pr.block_size = block_size
-    _lib.check(lib.ps_cascade_plan_build(ctypes.byref(pr), int(min_shared_pages),
-                                         plan.buffer.data_ptr(), plan.nbytes,
-                                         _stream_ptr(seq_lens.device)))
+    _launch(seq_lens.device, lib.ps_cascade_plan_build, ctypes.byref(pr), int(min_shared_pages),
+            plan.buffer.data_ptr(), plan.nbytes, _stream_ptr(seq_lens.device))
     plan.num_seqs = B
     return plan
 
@@ -607,13 +606,11 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
     if head_gather is not None:
         if cascade is not None or out_address is not None:
             raise ValueError("the fused head gather runs the plain decode into its own output")
-        _lib.check(lib.ps_paged_decode_head_gather(ctypes.byref(pr), workspace.buffer.data_ptr(),
-                                                   workspace.nbytes, ctypes.byref(head_gather),
-                                                   _stream_ptr(q.device)))
+        _launch(q.device, lib.ps_paged_decode_head_gather, ctypes.byref(pr), workspace.buffer.data_ptr(),
+                workspace.nbytes, ctypes.byref(head_gather), _stream_ptr(q.device))
     elif cascade is not None:
-        _lib.check(lib.ps_paged_decode_cascade(ctypes.byref(pr), cascade.buffer.data_ptr(),
-                                               cascade.nbytes, workspace.buffer.data_ptr(),
-                                               workspace.nbytes, _stream_ptr(q.device)))
+        _launch(q.device, lib.ps_paged_decode_cascade, ctypes.byref(pr), cascade.buffer.data_ptr(),
+                cascade.nbytes, workspace.buffer.data_ptr(), workspace.nbytes, _stream_ptr(q.device))
     elif score_mod is not None:
         mod = score_mod._struct(q, B)
         _launch(q.device, lib.ps_paged_decode_mod, ctypes.byref(pr), ctypes.byref(mod),
@@ -705,12 +702,12 @@ def merge_attn_states(output: torch.Tensor, prefix_output: torch.Tensor, prefix_
     for t in (prefix_lse, suffix_lse) + ((output_lse,) if output_lse is not None else ()):
         if t.dtype != torch.float32 or tuple(t.shape) != (H, T) or not t.is_contiguous():
             raise ValueError("LSEs must be contiguous float32 [H, T]")
-    _lib.check(lib.ps_merge_attn_states(
-        prefix_output.data_ptr(), prefix_output.stride(0), prefix_output.stride(1), prefix_lse.data_ptr(),
-        suffix_output.data_ptr(), suffix_output.stride(0), suffix_output.stride(1), suffix_lse.data_ptr(),
-        output.data_ptr(), output.stride(0), output.stride(1),
-        output_lse.data_ptr() if output_lse is not None else None,
-        T, H, D, _DTYPES[output.dtype], _stream_ptr(output.device)))
+    _launch(output.device, lib.ps_merge_attn_states,
+            prefix_output.data_ptr(), prefix_output.stride(0), prefix_output.stride(1), prefix_lse.data_ptr(),
+            suffix_output.data_ptr(), suffix_output.stride(0), suffix_output.stride(1), suffix_lse.data_ptr(),
+            output.data_ptr(), output.stride(0), output.stride(1),
+            output_lse.data_ptr() if output_lse is not None else None,
+            T, H, D, _DTYPES[output.dtype], _stream_ptr(output.device))
     return output
 
 
@@ -750,10 +747,10 @@ def chunked_prefill(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
                 workspace.buffer.data_ptr() if workspace is not None else None,
                 workspace.nbytes if workspace is not None else 0, _stream_ptr(q.device))
     elif workspace is not None:
-        _lib.check(lib.ps_chunked_prefill_ws(ctypes.byref(pr), workspace.buffer.data_ptr(),
-                                             workspace.nbytes, _stream_ptr(q.device)))
+        _launch(q.device, lib.ps_chunked_prefill_ws, ctypes.byref(pr), workspace.buffer.data_ptr(),
+                workspace.nbytes, _stream_ptr(q.device))
     else:
-        _lib.check(lib.ps_chunked_prefill(ctypes.byref(pr), _stream_ptr(q.device)))
+        _launch(q.device, lib.ps_chunked_prefill, ctypes.byref(pr), _stream_ptr(q.device))
     return out
 
 
