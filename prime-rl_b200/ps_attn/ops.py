@@ -481,14 +481,26 @@ def _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
         raise ValueError("block_table rows and seq_lens must be contiguous")
     if q.stride(-1) != 1 or out.stride(-1) != 1 or key_cache.stride(-1) != 1:
         raise ValueError("last dimension must be contiguous")
-    if lse is not None and lse.dtype != torch.float32:
-        raise ValueError("lse must be float32 [num_q_heads, num_tokens]")
+    rows, hq, dq = q.shape
     nb, bs, hkv, d = key_cache.shape
     if fp4:
-        nb, hkv, bs, d = key_cache.shape[0], key_cache.shape[1], key_cache.shape[2], q.shape[-1]
-    hq = q.shape[1]
-    if out.shape[0] < q.shape[0]:
-        raise ValueError("out has fewer rows than q")
+        hkv, bs, d = bs, hkv, dq
+    if d != dq:
+        raise ValueError(f"q has head size {dq}, the cache {d}")
+    if out.shape[0] < rows or out.shape[1:] != q.shape[1:]:
+        raise ValueError("out must have q's heads and head size, and no fewer rows than q")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape[0] < hq or lse.shape[1] < rows):
+        raise ValueError("lse must be float32 [num_q_heads, num_tokens]")
+    # (the kernels read a table row and an offset, or a query row, per sequence)
+    num_seqs = seq_lens.shape[0]
+    table_rows, table_cols = block_table.shape
+    if table_rows < num_seqs:
+        raise ValueError(f"block_table has {table_rows} rows for {num_seqs} sequences")
+    if query_start_loc is None:
+        if rows < num_seqs:
+            raise ValueError(f"q has {rows} rows for {num_seqs} sequences")
+    elif query_start_loc.shape[0] <= num_seqs or not query_start_loc.is_contiguous():
+        raise ValueError(f"query_start_loc must be contiguous, with {num_seqs + 1} entries")
     if status is not None and (status.dtype != torch.int32 or not status.is_cuda):
         raise ValueError("status must be a CUDA int32 tensor")
     q_st, q_sh = q.stride()[:2]
@@ -501,10 +513,10 @@ def _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
     # packed in one go: setting the fields one by one costs a small call 8 us
     return _lib.PagedProblem.from_buffer_copy(_lib.PAGED_PROBLEM_STRUCT.pack(
         q.data_ptr(), q_st, q_sh, key_cache.data_ptr(), value_cache.data_ptr(), s_block, s_slot, s_head, nb,
-        block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
-        query_start_loc.data_ptr() if query_start_loc is not None else 0, seq_lens.shape[0],
+        block_table.data_ptr(), block_table.stride(0), table_cols, seq_lens.data_ptr(),
+        query_start_loc.data_ptr() if query_start_loc is not None else 0, num_seqs,
         out.data_ptr(), o_st, o_sh, lse.data_ptr() if lse is not None else 0, l_sh, l_st,
-        hq, hkv, d, bs, _DTYPES[q.dtype], float(softmax_scale), q.shape[0],
+        hq, hkv, d, bs, _DTYPES[q.dtype], float(softmax_scale), rows,
         status.data_ptr() if status is not None else 0,
         0, 0, 0, 0, 0, 0, 0,  # new_key .. slot_mapping: set by the caller
         _lib.PS_KV_NVFP4 if fp4 else _lib.PS_KV_FP8_E4M3 if fp8 else _lib.PS_KV_AUTO,
@@ -596,7 +608,7 @@ def paged_decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Te
             raise ValueError("new key/value shape does not match the cache")
         if new_key.stride(-1) != 1 or new_value.stride(-1) != 1:
             raise ValueError("last dimension must be contiguous")
-        if slot_mapping.shape[0] < q.shape[0] or new_key.shape[0] < q.shape[0]:
+        if min(slot_mapping.shape[0], new_key.shape[0], new_value.shape[0]) < q.shape[0]:
             raise ValueError("fused append needs a key/value row and a slot per query row")
         pr.new_key = new_key.data_ptr()
         pr.new_key_stride_token, pr.new_key_stride_head = new_key.stride(0), new_key.stride(1)
@@ -666,6 +678,8 @@ def dequant_gather(key_cache: torch.Tensor, value_cache: torch.Tensor, block_tab
         raise ValueError("key_cache and value_cache must have the same shape and strides")
     if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
         raise ValueError("block_table and seq_lens must be int32")
+    if block_table.shape[0] < B:
+        raise ValueError(f"block_table has {block_table.shape[0]} rows for {B} sequences")
     if block_table.stride(-1) != 1 or not seq_lens.is_contiguous() or key_cache.stride(-1) != 1:
         raise ValueError("block_table rows, seq_lens and the caches' last dimension must be contiguous")
     if status is not None and (status.dtype != torch.int32 or not status.is_cuda):

@@ -72,3 +72,44 @@ def test_every_call_makes_its_device_current(trace):
     ops.rope_kv_append(q, k, k, slots, t(16, 128), True, kc, kc, slots)
     assert len(trace.calls) == 19
     assert [c for c in trace.calls if c[1] != 3] == [] and trace.current == 0
+
+
+SHORT = {
+    "table rows": (dict(bt=lambda x: x[:1]), "block_table has 1 rows"),
+    "query rows": (dict(q=lambda x: x[:1], out=lambda x: x[:1]), "q has 1 rows"),
+    "query offsets": (dict(qsl=lambda x: x[:2]), "3 entries"),
+    "strided query offsets": (dict(qsl=lambda x: t(6, dtype=torch.int32)[::2]), "3 entries"),
+    "head size": (dict(q=lambda x: t(2, 4, 64), out=lambda x: t(2, 4, 64)), "head size"),
+    "output heads": (dict(out=lambda x: t(2, 2, 128)), "out must have"),
+    "output head size": (dict(out=lambda x: t(2, 4, 64)), "out must have"),
+    "LSE heads": (dict(lse=lambda x: t(3, 2, dtype=torch.float32)), "lse"),
+    "LSE rows": (dict(lse=lambda x: t(4, 1, dtype=torch.float32)), "lse"),
+    "new values": (dict(nv=lambda x: x[:1]), "per query row"),
+}
+
+
+@pytest.mark.parametrize("what", SHORT)
+@pytest.mark.parametrize("kind", ["16bit", "nvfp4"])
+def test_arrays_shorter_than_the_kernels_read_are_refused(trace, what, kind):
+    if kind == "nvfp4" and what == "head size":
+        pytest.skip("a cache of its shape is not a 4-bit one for this head size")
+    a = dict(q=t(2, 4, 128), bt=t(2, 2, dtype=torch.int32), n=t(2, dtype=torch.int32), out=t(2, 4, 128), qsl=None,
+             lse=t(4, 2, dtype=torch.float32), nk=t(2, 2, 128), nv=t(2, 2, 128), slots=t(2, dtype=torch.int64))
+    if "offsets" in what:
+        a["qsl"] = t(3, dtype=torch.int32)
+    cache = t(3, 16, 2, 128) if kind == "16bit" else t(3, 2, 16, 72, dtype=torch.uint8)
+    ws = SimpleNamespace(max_num_seqs=8, num_kv_heads=2, nbytes=256, buffer=t(256, dtype=torch.uint8))
+
+    def go(a):
+        ops.paged_decode(a["q"], cache, cache, a["bt"], a["n"], 0.1, a["out"], lse=a["lse"], query_start_loc=a["qsl"],
+                         workspace=ws, new_key=a["nk"], new_value=a["nv"], slot_mapping=a["slots"])
+
+    go(a)
+    changes, match = SHORT[what]
+    with pytest.raises(ValueError, match=match):
+        go({k: changes[k](v) if k in changes else v for k, v in a.items()})
+    assert len(trace.calls) == 1
+    if what == "table rows" and kind == "nvfp4":
+        with pytest.raises(ValueError, match=match):
+            ops.dequant_gather(cache, cache, a["bt"][:1], a["n"], 2, torch.bfloat16,
+                               out=(t(4, 16, 2, 128), t(4, 16, 2, 128)))
