@@ -150,6 +150,7 @@ class PSAttentionMetadata:
     workspace: ops.DecodeWorkspace
     causal: bool = True
     cascade_plan: ops.CascadePlan | None = None  # shared-prefix plan of the decode rows
+    max_prefill_len: int = 0                     # of the prefill requests alone; 0: max_seq_len
     dcp_comm: object | None = None               # decode context parallel group (ps_attn.dcp.DcpComm)
 
 
@@ -208,12 +209,17 @@ class PSAttentionMetadataBuilder(AttentionMetadataBuilder[PSAttentionMetadata]):
             plan = ops.cascade_plan(m.block_table_tensor[:nd], m.seq_lens[:nd], self.num_heads_q,
                                     self.num_heads_kv, self.block_size,
                                     query_start_loc=m.query_start_loc[:nd + 1], plan=self.plan)
+        # what a quantized cache's prefill scratch has to hold: the longest prefill
+        # request, not the longest decode beside it (a host-side bound, where the
+        # step has one)
+        bound = getattr(m, "seq_lens_cpu_upper_bound", None)
+        longest = int(bound[nd:nd + npf].max()) if bound is not None and npf > 0 else 0
         return PSAttentionMetadata(
             num_actual_tokens=m.num_actual_tokens, max_query_len=m.max_query_len,
             query_start_loc=m.query_start_loc, max_seq_len=m.max_seq_len, seq_lens=m.seq_lens,
             block_table=m.block_table_tensor, slot_mapping=m.slot_mapping, num_decodes=nd,
             num_decode_tokens=ndt, num_prefills=npf, workspace=self.workspace, causal=True,
-            cascade_plan=plan, dcp_comm=getattr(self, "dcp_comm", None))
+            cascade_plan=plan, max_prefill_len=min(longest, m.max_seq_len), dcp_comm=getattr(self, "dcp_comm", None))
 
     def update_block_table(self, metadata: PSAttentionMetadata, blk_table: torch.Tensor,
                            slot_mapping: torch.Tensor) -> PSAttentionMetadata:
@@ -328,8 +334,9 @@ class PSAttentionImpl(AttentionImpl):
                 # scale) values exactly, unscaled, with the tensors' scales
                 # applied in the kernel
                 bs = key_cache.shape[2] if self.nvfp4 else key_cache.shape[1]
+                longest = m.max_prefill_len or m.max_seq_len
                 kc, vc, bt = ops.dequant_gather(key_cache, value_cache, bt, m.seq_lens[nd:],
-                                                (m.max_seq_len + bs - 1) // bs, query.dtype)
+                                                (longest + bs - 1) // bs, query.dtype)
             ops.chunked_prefill(query[:T], kc, vc, bt, m.seq_lens[nd:], m.query_start_loc[nd:],
                                 self.scale, output[:T], workspace=m.workspace, score_mod=mod, **sc)
         return output

@@ -28,6 +28,39 @@ def test_impls_take_a_layers_positional_arguments(cls):
         cls(HQ, D, 0.088, HKV, None, None, "auto", None, "encoder", None)
 
 
+def common(qlens, lens, bound):
+    from vllm.v1.attention.backend import CommonAttentionMetadata
+
+    qsl = torch.tensor([0] + qlens).cumsum(0).int()
+    return CommonAttentionMetadata(
+        query_start_loc=qsl, query_start_loc_cpu=qsl.clone(), seq_lens=torch.tensor(lens, dtype=torch.int32),
+        num_reqs=len(qlens), num_actual_tokens=sum(qlens), max_query_len=max(qlens), max_seq_len=max(lens),
+        block_table_tensor=torch.zeros(len(qlens), 2048, dtype=torch.int32),
+        slot_mapping=torch.arange(sum(qlens)), seq_lens_cpu_upper_bound=bound)
+
+
+@pytest.mark.parametrize("dtype", ["nvfp4", "fp8"])
+def test_prefill_scratch_holds_the_prefills_not_the_longest_decode(monkeypatch, dtype):
+    """Two short prompts beside a decode of 32,000 tokens: scratch for the prompts' pages, where the step's lengths
+    are known on the host."""
+    calls = []
+    for name in ("kv_append", "paged_decode", "chunked_prefill"):
+        monkeypatch.setattr(psb.ops, name, lambda *a, **k: None)
+    monkeypatch.setattr(psb.ops, "dequant_gather", lambda *a, **k: calls.append(a) or ("k", "v", "bt"))
+    impl = psb.PSAttentionImpl(HQ, D, 0.088, HKV, None, None, dtype)
+    kv = torch.zeros(psb.PSAttentionBackend.get_kv_cache_shape(4, BS, HKV, D, dtype), dtype=torch.uint8)
+    q = torch.zeros(71, HQ, D)
+    builder = psb.PSAttentionMetadataBuilder.__new__(psb.PSAttentionMetadataBuilder)
+    builder.workspace = object()
+    lens = [32_000, 50, 70]
+    for bound, pages in ((torch.tensor([32_001, 50, 71]), 5), (None, 2000)):
+        md = builder.build(0, common([1, 50, 20], lens, bound))
+        impl.forward(object(), q, q[:, :HKV], q[:, :HKV], kv, md, torch.zeros_like(q))
+        assert calls.pop()[4] == pages
+    # a decode-only step has no prefill
+    assert builder.build(0, common([1, 1], [5, 6], torch.tensor([5, 6]))).max_prefill_len == 0
+
+
 CASES = {
     "nvfp4": ("nvfp4", {}, {}),
     "nvfp4_window_cap": ("nvfp4", dict(per_layer_sliding_window=100, logits_soft_cap=20.0),
