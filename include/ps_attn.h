@@ -265,8 +265,10 @@ typedef struct {
   const float* alibi_slopes;  /* device [num_q_heads], NULL: no bias */
   int32_t window_left;        /* < 0: no window */
   const int32_t* key_start;   /* device, per query row (num_tokens entries), NULL: 0 */
-  const int32_t* prefix_lens; /* device [num_seqs], NULL: causal.  A decode row sees
-                                 every key up to its own already: no effect there */
+  const int32_t* prefix_lens; /* device [num_seqs], NULL: causal.  Rows before a
+                                 prefix's end see its later keys too (the window and
+                                 key_start cut them as they cut any).  A decode row
+                                 has none: no effect there */
 } ps_score_mod;
 
 /* ps_paged_decode with score modifiers, over 16-bit, fp8 and nvfp4 caches, the

@@ -7,7 +7,7 @@
 //
 // Layout: a cache half is [num_blocks][num_kv_heads][block_size][72] bytes, in
 // which the 16 tokens of a page of one head are one contiguous 1152-byte tile
-// (a single bulk copy), ordered for the decode's tensor-core fragments so that
+// (copied 16 bytes a lane), ordered for the decode's tensor-core fragments so that
 // a lane's operands are two 16-byte shared-memory loads:
 //   K tile: codes of token r, dims d, d + 1 (d even; d in the low nibble) at
 //           r * 64 + d / 2; scale of block k at 1024 + r * 8 + k.  A lane

@@ -1,8 +1,9 @@
 // Launches of the paged split-KV decode with score modifiers: tanh cap, bias
 // that falls with the distance, sliding window, document mask.  The kernel is
 // paged_decode_impl.cuh's in its kModded mode: the page-head list holds only
-// the units from each sequence's first visible key on, so a sliding window
-// reads window / 16 + 1 pages of a sequence however long it is.
+// the units from each sequence's first visible key on, so a sliding window of
+// window_left = W (W + 1 keys) reads at most (W + 15) / 16 + 1 pages of a sequence
+// however long it is.
 #include "paged_decode_impl.cuh"
 
 namespace ps {

@@ -123,7 +123,8 @@ int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 // kind with any batch size up to the one it was sized for:
 //   [0, 256)                 status word; bytes 16..23: prefill unit scheduler
 //   [256, 256 + C)           counters, kDecodeMaxSeqs * num_kv_heads int32
-//   [.., + C)                prefix-segment counters (cascade)
+//   [.., + C)                prefix-segment counters (cascade), or two counters per
+//                            warp for merges in two levels (score modifiers, 4 bit)
 //   [..., ...)               partial records, one per split slot:
 //                            kg * 128 fp32 output rows, then kg fp32 LSEs
 //                            (kg = 8 or 16 by GQA group; 16 in cascade mode)
@@ -268,12 +269,16 @@ int decode_impl(const ps_paged_problem* pr, const void* plan, int64_t plan_bytes
   const bool fp8 = pr->kv_cache_dtype == PS_KV_FP8_E4M3;
   const bool fp4 = pr->kv_cache_dtype == PS_KV_NVFP4;
   if (fp8 && cascade) return fail(PS_ERR_UNSUPPORTED, "cascade decode over an fp8 cache is not built");
+  if ((fp4 || mod != nullptr) &&
+      2LL * sms * ps::kDecodeCtasPerSm * (fp4 ? ps::kDecodeFp4Warps : ps::kDecodeMaxWarps) >
+          static_cast<int64_t>(ps::kDecodeMaxSeqs) * pr->num_kv_heads)
+    return fail(PS_ERR_UNSUPPORTED, "%d SMs: more merge counters than the workspace has", sms);
   const DecodeWorkspaceLayout lay =
       decode_layout(pr->num_seqs, pr->num_q_heads, pr->num_kv_heads, sms, cascade, fp8, fp4);
   if (!workspace || workspace_bytes < lay.total || !aligned(workspace, 256))
     return fail(PS_ERR_WORKSPACE, "decode workspace must be >= %lld bytes, 256-byte aligned",
                 static_cast<long long>(lay.total));
-  CUtensorMap kmap, vmap;  // (nvfp4 tiles are contiguous: plain bulk copies)
+  CUtensorMap kmap, vmap;  // (nvfp4 tiles are contiguous: copied 16 bytes a lane)
   if (!fp4) {
     rc = make_page_map(&kmap, pr->key_cache, pr->num_blocks, pr->block_size, pr->num_kv_heads,
                        pr->cache_stride_block, pr->cache_stride_slot, pr->cache_stride_head, fp8 ? 1 : 2);

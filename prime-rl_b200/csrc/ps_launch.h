@@ -31,7 +31,7 @@ struct ScoreModParams {
   const float* slopes;       // [num_q_heads] bias slopes; nullptr: none
   int32_t window_left;       // keys j >= i - window_left; < 0: no window
   const int32_t* key_start;  // [query rows] first key of the row's document; nullptr: 0
-  const int32_t* prefix_lens;  // [num_seqs] keys every row sees; nullptr: causal (prefill)
+  const int32_t* prefix_lens;  // [num_seqs] keys that are visible also to the rows before them; nullptr: causal (prefill)
 };
 
 // Paged decode launch parameters (device-visible copy of ps_paged_problem plus

@@ -111,9 +111,10 @@ class ScoreMod:
 
     alibi_slopes: float32 [Hq]; window_left: -1 for no window (vLLM's
     ``sliding_window - 1``); key_start: int32, one entry per query row, the
-    first key of the row's document; prefix_lens: int32 [B], the keys every row
-    of the sequence sees (prefill; no effect on a decode row, which sees all
-    keys up to its own).  Keys past a row's range may hold anything; keys that
+    first key of the row's document; prefix_lens: int32 [B], the first keys of
+    the sequence, which the rows before them see too, as far as the window and
+    ``key_start`` let them (prefill; no effect on a decode row, which sees no
+    key behind its own).  Keys past a row's range may hold anything; keys that
     one row of a sequence sees and another does not must hold finite values.
     """
 
