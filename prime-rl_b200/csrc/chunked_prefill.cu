@@ -5,6 +5,9 @@
 int ps_launch_chunked_prefill(const ps::PrefillParams& p, const CUtensorMap& qmap,
                               const CUtensorMap& kmap, const CUtensorMap& vmap, int dtype_bf16,
                               int grid, cudaStream_t stream) {
+  if (p.k_scale != nullptr || p.v_scale != nullptr)
+    return dtype_bf16 ? ps::launch_prefill_t<true, false, false, false, true>(p, qmap, kmap, vmap, grid, stream)
+                      : ps::launch_prefill_t<false, false, false, false, true>(p, qmap, kmap, vmap, grid, stream);
   return dtype_bf16 ? ps::launch_prefill_t<true>(p, qmap, kmap, vmap, grid, stream)
                     : ps::launch_prefill_t<false>(p, qmap, kmap, vmap, grid, stream);
 }

@@ -80,8 +80,10 @@ __device__ __forceinline__ float exp2_fma(float x) {
 }
 
 // The same with a quartic (max relative error 2.6e-6), for the kernels with score
-// modifiers.  One score in eight takes it: with the cubic the row sums, and so
-// the LSEs, were 1e-6 off.
+// modifiers and for calls with cache scales, which are over the pages of a quantized
+// cache.  One score in eight takes it: with the cubic the row sums, and so the
+// LSEs, were up to 4e-5 off.  (24 turns of 77 rows: 72.5
+// -> 73.3 us; four chunks of 1,024: 336 either way.)
 __device__ __forceinline__ float exp2_fma4(float x) {
   const float xc = fmaxf(x, -127.f);
   const float t = xc + 12582912.f;
@@ -309,7 +311,7 @@ __device__ __forceinline__ int next_unit(const PrefillParams& p, const PBars& ba
   return nxt;
 }
 
-template <bool kBF16, bool kMod = false, bool kCap = false, bool kBias = false>
+template <bool kBF16, bool kMod = false, bool kCap = false, bool kBias = false, bool kFine = kMod>
 __global__ void __launch_bounds__(kThreads, 1)
     chunked_prefill_kernel(const __grid_constant__ PrefillParams p,
                            const __grid_constant__ CUtensorMap qmap,
@@ -822,8 +824,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               float x0, x1;
               const uint64_t y2 = f2_pack(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1]));
               f2_unpack(kCap || kBias ? f2_add(y2, negm_x2) : f2_fma(y2, sl2x2, negm_x2), x0, x1);
-              const float p0 = (2 * i) % 8 >= PS_PREFILL_EMU_PER8 ? ex2(x0) : kMod ? exp2_fma4(x0) : exp2_fma(x0);
-              const float p1 = (2 * i + 1) % 8 >= PS_PREFILL_EMU_PER8 ? ex2(x1) : kMod ? exp2_fma4(x1) : exp2_fma(x1);
+              const float p0 = (2 * i) % 8 >= PS_PREFILL_EMU_PER8 ? ex2(x0) : kFine ? exp2_fma4(x0) : exp2_fma(x0);
+              const float p1 = (2 * i + 1) % 8 >= PS_PREFILL_EMU_PER8 ? ex2(x1) : kFine ? exp2_fma4(x1) : exp2_fma(x1);
               rsp[i & 3] = f2_add(rsp[i & 3], f2_pack(p0, p1));
               pk[i] = pack2<kBF16>(p0, p1);
             }
@@ -1010,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <bool kBF16, bool kMod = false, bool kCap = false, bool kBias = false>
+template <bool kBF16, bool kMod = false, bool kCap = false, bool kBias = false, bool kFine = kMod>
 static int launch_prefill_t(const PrefillParams& p, const CUtensorMap& qmap, const CUtensorMap& kmap,
                             const CUtensorMap& vmap, int grid, cudaStream_t stream) {
   const size_t smem = 1024 + PrefillSmem::bytes_before_table + static_cast<size_t>(p.num_seqs + 1) * 4;
@@ -1019,7 +1021,7 @@ static int launch_prefill_t(const PrefillParams& p, const CUtensorMap& qmap, con
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return static_cast<int>(cudaErrorInvalidDevice);
   if (!configured[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(
-        chunked_prefill_kernel<kBF16, kMod, kCap, kBias>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        chunked_prefill_kernel<kBF16, kMod, kCap, kBias, kFine>, cudaFuncAttributeMaxDynamicSharedMemorySize,
         static_cast<int>(1024 + PrefillSmem::bytes_before_table + (kPrefillMaxSeqs + 1) * 4));
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev] = true;
@@ -1034,7 +1036,7 @@ static int launch_prefill_t(const PrefillParams& p, const CUtensorMap& qmap, con
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunked_prefill_kernel<kBF16, kMod, kCap, kBias>, p, qmap, kmap, vmap);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, chunked_prefill_kernel<kBF16, kMod, kCap, kBias, kFine>, p, qmap, kmap, vmap);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 

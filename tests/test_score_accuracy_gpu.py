@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import mod_ref
+from ps_attn import ops
 from test_score_mod_gpu import run_decode, run_prefill, slopes
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +94,15 @@ def test_decode_lse(name, kind):
     b = mod_ref.Batch(lens, [1] * 5, 8, 2, kind=kind, seed=62)
     m = mods(8, [1] * 5, lens)[name]
     check(run_decode(b, m)[1], reference(b, m, False))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["fp8", "nvfp4"])
+def test_prefill_lse_over_a_quantized_cache(kind, dtype):
+    """Rows of few keys among them, whose sums a coarse exponential of one key in eight would show in."""
+    rows, lens = [25, 1, 60, 3, 90], [25, 31, 200, 400, 90]
+    b = mod_ref.Batch(lens, rows, 4, 2, dtype=dtype, kind=kind, seed=63)
+    k, v, table = ops.dequant_gather(b.kc, b.vc, b.table, b.lens, b.table.shape[1], b.dtype)
+    out, lse = torch.empty_like(b.q), torch.empty(4, sum(rows), device="cuda")
+    ops.chunked_prefill(b.q, k, v, table, b.lens, b.starts.cuda(), b.scale, out, lse=lse, **b.scales)
+    check(lse, reference(b, {}, True))
