@@ -459,42 +459,56 @@ def cascade_plan(block_table: torch.Tensor, seq_lens: torch.Tensor, num_q_heads:
 def _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
              softmax_scale, out, lse, status=None, k_scale=None, v_scale=None) -> _lib.PagedProblem:
     _require_cuda(q, key_cache, value_cache, block_table, seq_lens, out, query_start_loc, lse)
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"attention dtype {q.dtype} unsupported (fp16/bf16)")
-    fp4 = is_nvfp4_cache(key_cache, q.shape[-1])
-    fp8 = is_fp8_cache(key_cache) and not fp4
+    # (shapes and strides are read once each: a read costs 0.1-0.2 us of a small call)
+    dtype = q.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"attention dtype {dtype} unsupported (fp16/bf16)")
+    rows, hq, dq = q.shape
+    q_st, q_sh, q_sd = q.stride()
+    out_rows, out_heads, out_d = out.shape
+    o_st, o_sh, o_sd = out.stride()
+    cache_dtype = key_cache.dtype
+    fp4 = is_nvfp4_cache(key_cache, dq)
+    fp8 = cache_dtype in FP8_CACHE_DTYPES and not fp4
     if fp4:
         _check_nvfp4(key_cache, value_cache)
-        if out.dtype != q.dtype:
+        if out.dtype != dtype:
             raise ValueError("nvfp4 cache: out must have the query dtype")
     elif fp8:
-        if value_cache.dtype != key_cache.dtype or out.dtype != q.dtype:
+        if value_cache.dtype != cache_dtype or out.dtype != dtype:
             raise ValueError("fp8 cache: both caches fp8, out in the query dtype")
-    elif key_cache.dtype != q.dtype or value_cache.dtype != q.dtype or out.dtype != q.dtype:
+    elif cache_dtype != dtype or value_cache.dtype != dtype or out.dtype != dtype:
         raise ValueError("q, caches and out must share one dtype")
-    if key_cache.stride() != value_cache.stride() or key_cache.shape != value_cache.shape:
+    strides = key_cache.stride()
+    if strides != value_cache.stride() or key_cache.shape != value_cache.shape:
         raise ValueError("key_cache and value_cache must have the same shape and strides")
     if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
         raise ValueError("block_table and seq_lens must be int32")
     if query_start_loc is not None and query_start_loc.dtype != torch.int32:
         raise ValueError("query_start_loc must be int32")
-    if block_table.stride(-1) != 1 or not seq_lens.is_contiguous():
+    table_rows, table_cols = block_table.shape
+    table_st, table_sd = block_table.stride()
+    if table_sd != 1 or not seq_lens.is_contiguous():
         raise ValueError("block_table rows and seq_lens must be contiguous")
-    if q.stride(-1) != 1 or out.stride(-1) != 1 or key_cache.stride(-1) != 1:
+    if q_sd != 1 or o_sd != 1 or strides[3] != 1:
         raise ValueError("last dimension must be contiguous")
-    rows, hq, dq = q.shape
     nb, bs, hkv, d = key_cache.shape
+    s_block, s_slot, s_head = strides[:3]
     if fp4:
         hkv, bs, d = bs, hkv, dq
+        s_slot, s_head = s_head, s_slot
     if d != dq:
         raise ValueError(f"q has head size {dq}, the cache {d}")
-    if out.shape[0] < rows or out.shape[1:] != q.shape[1:]:
+    if out_rows < rows or out_heads != hq or out_d != dq:
         raise ValueError("out must have q's heads and head size, and no fewer rows than q")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape[0] < hq or lse.shape[1] < rows):
-        raise ValueError("lse must be float32 [num_q_heads, num_tokens]")
+    l_sh = l_st = 0
+    if lse is not None:
+        lse_heads, lse_rows = lse.shape
+        if lse.dtype != torch.float32 or lse_heads < hq or lse_rows < rows:
+            raise ValueError("lse must be float32 [num_q_heads, num_tokens]")
+        l_sh, l_st = lse.stride()
     # (the kernels read a table row and an offset, or a query row, per sequence)
     num_seqs = seq_lens.shape[0]
-    table_rows, table_cols = block_table.shape
     if table_rows < num_seqs:
         raise ValueError(f"block_table has {table_rows} rows for {num_seqs} sequences")
     if query_start_loc is None:
@@ -504,20 +518,13 @@ def _problem(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
         raise ValueError(f"query_start_loc must be contiguous, with {num_seqs + 1} entries")
     if status is not None and (status.dtype != torch.int32 or not status.is_cuda):
         raise ValueError("status must be a CUDA int32 tensor")
-    q_st, q_sh = q.stride()[:2]
-    o_st, o_sh = out.stride()[:2]
-    if fp4:
-        s_block, s_head, s_slot = key_cache.stride()[:3]
-    else:
-        s_block, s_slot, s_head = key_cache.stride()[:3]
-    l_sh, l_st = (lse.stride(0), lse.stride(1)) if lse is not None else (0, 0)
     # packed in one go: setting the fields one by one costs a small call 8 us
     return _lib.PagedProblem.from_buffer_copy(_lib.PAGED_PROBLEM_STRUCT.pack(
         q.data_ptr(), q_st, q_sh, key_cache.data_ptr(), value_cache.data_ptr(), s_block, s_slot, s_head, nb,
-        block_table.data_ptr(), block_table.stride(0), table_cols, seq_lens.data_ptr(),
+        block_table.data_ptr(), table_st, table_cols, seq_lens.data_ptr(),
         query_start_loc.data_ptr() if query_start_loc is not None else 0, num_seqs,
         out.data_ptr(), o_st, o_sh, lse.data_ptr() if lse is not None else 0, l_sh, l_st,
-        hq, hkv, d, bs, _DTYPES[q.dtype], float(softmax_scale), rows,
+        hq, hkv, d, bs, _DTYPES[dtype], float(softmax_scale), rows,
         status.data_ptr() if status is not None else 0,
         0, 0, 0, 0, 0, 0, 0,  # new_key .. slot_mapping: set by the caller
         _lib.PS_KV_NVFP4 if fp4 else _lib.PS_KV_FP8_E4M3 if fp8 else _lib.PS_KV_AUTO,
