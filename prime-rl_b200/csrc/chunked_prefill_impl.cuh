@@ -663,13 +663,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             // (minimax, relative error 5.4e-7): five packed instructions for two
             // scores on the FMA pipe, where exp and reciprocal take four turns
             // of the MUFU unit, which sets the pace of a tile.  Window and cap on
-            // 13,000 prompt tokens, 32 / 8 heads: 391 us, 493 with the
+            // 13,000 prompt tokens, 32 / 8 heads: 385 us, 493 with the
             // exponential for every score, 285 without a cap.  (A quadratic for
             // z up to c / 4 gained 1 %.)  A warp with a score beyond takes both
             // forms and each score its own, so that what a score becomes depends on
             // nothing else: not on the row's other scores (the exponential's error,
             // 2^-22 c, is too much for small ones), nor on what lies in keys that no
-            // row sees.  (Registers for that: 14 of the 391 us.)
+            // row sees.  (Registers and code for that: 7 of the 385 us;
+            // 14 with the branches the other way round.)
             float am[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -678,22 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 am[i & 3] = max3(am[i & 3], fabsf(__uint_as_float(r[c][2 * i])), fabsf(__uint_as_float(r[c][2 * i + 1])));
             // (a NaN, in keys past the range or not, stays a NaN either way)
             const float amax = fmaxf(max3(am[0], am[1], am[2]), am[3]);
-            if (__all_sync(0xffffffffu, amax <= cap_fast)) {
-              const float a2 = cap_u * cap_u, k0 = sl2 * 0.99999946f, k1 = -0.3332632f * (sl2 * a2);
-              const float k2 = 0.13190296f * (sl2 * a2) * a2, k3 = -0.044402227f * (sl2 * a2) * a2 * a2;
-              const uint64_t q0 = f2_pack(k0, k0), q1 = f2_pack(k1, k1), q2 = f2_pack(k2, k2), q3 = f2_pack(k3, k3);
-#pragma unroll
-              for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const uint64_t v = f2_pack(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1]));
-                  const uint64_t v2 = f2_mul(v, v);
-                  float y0, y1;
-                  f2_unpack(f2_mul(v, f2_fma(f2_fma(f2_fma(q3, v2, q2), v2, q1), v2, q0)), y0, y1);
-                  r[c][2 * i] = __float_as_uint(y0);
-                  r[c][2 * i + 1] = __float_as_uint(y1);
-                }
-            } else {
+            if (__builtin_expect(!__all_sync(0xffffffffu, amax <= cap_fast), 0)) {
               // the same polynomial in w = raw score * 2^n, z / c = cap_r w with
               // cap_r in [1/2, 1) (bit for bit what the other branch computes)
               const int e = min(max((__float_as_int(cap_u) >> 23) + 1, 27), 253);
@@ -717,6 +703,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const float f1 = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + ex2(w1 * far_in)), cap2);
                   r[c][2 * i] = __float_as_uint(fabsf(w0) * cap_r <= 0.5f ? y0 : f0);
                   r[c][2 * i + 1] = __float_as_uint(fabsf(w1) * cap_r <= 0.5f ? y1 : f1);
+                }
+            } else {
+
+              const float a2 = cap_u * cap_u, k0 = sl2 * 0.99999946f, k1 = -0.3332632f * (sl2 * a2);
+              const float k2 = 0.13190296f * (sl2 * a2) * a2, k3 = -0.044402227f * (sl2 * a2) * a2 * a2;
+              const uint64_t q0 = f2_pack(k0, k0), q1 = f2_pack(k1, k1), q2 = f2_pack(k2, k2), q3 = f2_pack(k3, k3);
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const uint64_t v = f2_pack(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1]));
+                  const uint64_t v2 = f2_mul(v, v);
+                  float y0, y1;
+                  f2_unpack(f2_mul(v, f2_fma(f2_fma(f2_fma(q3, v2, q2), v2, q1), v2, q0)), y0, y1);
+                  r[c][2 * i] = __float_as_uint(y0);
+                  r[c][2 * i + 1] = __float_as_uint(y1);
                 }
             }
           }
