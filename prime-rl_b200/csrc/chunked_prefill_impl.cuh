@@ -705,7 +705,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                   r[c][2 * i + 1] = __float_as_uint(fabsf(w1) * cap_r <= 0.5f ? y1 : f1);
                 }
             } else {
-
               const float a2 = cap_u * cap_u, k0 = sl2 * 0.99999946f, k1 = -0.3332632f * (sl2 * a2);
               const float k2 = 0.13190296f * (sl2 * a2) * a2, k3 = -0.044402227f * (sl2 * a2) * a2 * a2;
               const uint64_t q0 = f2_pack(k0, k0), q1 = f2_pack(k1, k1), q2 = f2_pack(k2, k2), q3 = f2_pack(k3, k3);

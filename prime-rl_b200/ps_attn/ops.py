@@ -777,11 +777,15 @@ def chunked_prefill(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
 
 
 def paged_attention(q, key_cache, value_cache, out, query_start_loc, max_query_len, seq_lens,
-                    softmax_scale, block_table, lse=None, workspace=None, score_mod=None):
-    """``flash_attn_varlen_func``'s paged, causal call shape: route by ``max_query_len``."""
+                    softmax_scale, block_table, lse=None, workspace=None, score_mod=None,
+                    k_scale=None, v_scale=None):
+    """``flash_attn_varlen_func``'s paged, causal call shape: route by ``max_query_len``.
+    ``k_scale`` / ``v_scale``: an fp8 or nvfp4 cache's (single-row calls), or those of the
+    cache that 16-bit pages were gathered from."""
     if max_query_len <= 1:
         return paged_decode(q, key_cache, value_cache, block_table, seq_lens, softmax_scale, out,
                             lse=lse, query_start_loc=query_start_loc, workspace=workspace,
-                            score_mod=score_mod)
+                            score_mod=score_mod, k_scale=k_scale, v_scale=v_scale)
     return chunked_prefill(q, key_cache, value_cache, block_table, seq_lens, query_start_loc,
-                           softmax_scale, out, lse=lse, score_mod=score_mod)
+                           softmax_scale, out, lse=lse, score_mod=score_mod, k_scale=k_scale,
+                           v_scale=v_scale)

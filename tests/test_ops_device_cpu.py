@@ -113,3 +113,12 @@ def test_arrays_shorter_than_the_kernels_read_are_refused(trace, what, kind):
         with pytest.raises(ValueError, match=match):
             ops.dequant_gather(cache, cache, a["bt"][:1], a["n"], 2, torch.bfloat16,
                                out=(t(4, 16, 2, 128), t(4, 16, 2, 128)))
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+def test_paged_attention_passes_the_scales_on(trace, monkeypatch, rows):
+    got = []
+    for name in ("paged_decode", "chunked_prefill"):
+        monkeypatch.setattr(ops, name, lambda *a, _n=name, **k: got.append((_n, k["k_scale"], k["v_scale"])))
+    ops.paged_attention("q", "k", "v", "o", None, rows, "n", 0.1, "bt", k_scale=2, v_scale=3)
+    assert got == [("paged_decode" if rows == 1 else "chunked_prefill", 2, 3)]
