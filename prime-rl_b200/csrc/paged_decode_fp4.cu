@@ -4,7 +4,8 @@
 //
 // A page-head is 2304 bytes (K tile + V tile) against 8192 in 16 bits, so
 // what bounds the kernel is the instruction stream that turns codes into
-// tensor-core operands, not HBM.  Hence:
+// tensor-core operands (each warp's own: 57 % of the issue slots are taken), not HBM.
+// Hence:
 //   - the unit of work is four pages of one (sequence, kv head): one wait, one
 //     maximum and one rescale per unit; four more warps of a CTA do the copying;
 //   - the tile layout (nvfp4.cuh) is the fragment order: a lane's K codes are
