@@ -213,7 +213,9 @@ class PSAttentionMetadataBuilder(AttentionMetadataBuilder[PSAttentionMetadata]):
         # request, not the longest decode beside it (a host-side bound, where the
         # step has one)
         bound = getattr(m, "seq_lens_cpu_upper_bound", None)
-        longest = int(bound[nd:nd + npf].max()) if bound is not None and npf > 0 else 0
+        longest = 0
+        if bound is not None and npf > 0 and bound.shape[0] >= nd + npf and not bound.is_cuda:
+            longest = int(bound[nd:nd + npf].max())
         return PSAttentionMetadata(
             num_actual_tokens=m.num_actual_tokens, max_query_len=m.max_query_len,
             query_start_loc=m.query_start_loc, max_seq_len=m.max_seq_len, seq_lens=m.seq_lens,

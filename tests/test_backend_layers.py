@@ -53,7 +53,8 @@ def test_prefill_scratch_holds_the_prefills_not_the_longest_decode(monkeypatch, 
     builder = psb.PSAttentionMetadataBuilder.__new__(psb.PSAttentionMetadataBuilder)
     builder.workspace = object()
     lens = [32_000, 50, 70]
-    for bound, pages in ((torch.tensor([32_001, 50, 71]), 5), (None, 2000)):
+    # (a bound for some of the requests only is none)
+    for bound, pages in ((torch.tensor([32_001, 50, 71]), 5), (None, 2000), (torch.tensor([32_001, 50]), 2000)):
         md = builder.build(0, common([1, 50, 20], lens, bound))
         impl.forward(object(), q, q[:, :HKV], q[:, :HKV], kv, md, torch.zeros_like(q))
         assert calls.pop()[4] == pages
